@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libflexhip.so")
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+DT_E4M3, DT_E5M2 = 3, 4
 ACT_SILU, ACT_GELU_TANH = 0, 1
 
 _DTYPE_ENUM = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
@@ -26,6 +27,17 @@ def dtype_enum(dtype: torch.dtype) -> int:
         return _DTYPE_ENUM[dtype]
     except KeyError:
         raise TypeError(f"dtype {dtype} not supported; supported: {list(_DTYPE_ENUM)}") from None
+
+
+_FP8_ENUM = {torch.float8_e4m3fn: DT_E4M3, torch.float8_e5m2: DT_E5M2}
+
+
+def fp8_enum(dtype: torch.dtype) -> int:
+    """3 e4m3 / 4 e5m2: the 8-bit value types of the block-scaled ops."""
+    try:
+        return _FP8_ENUM[dtype]
+    except KeyError:
+        raise TypeError(f"8-bit dtype {dtype} not supported; supported: {list(_FP8_ENUM)}") from None
 
 
 # name -> (restype, argtypes); one entry per declaration in include/flexhip.h
@@ -125,6 +137,26 @@ _SIGNATURES = {
     "solve_scheduler": (c_double, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_double, c_int, c_int,
                                    c_void_p]),
     "compute_buf_size": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_double, c_int]),
+    "fx_add_rmsnorm_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                   c_int64, c_int, c_float, c_int, c_int, c_int, c_void_p]),
+    "fx_add_rmsnorm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                   c_int64, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "fx_fp8_quantize": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_int64,
+                                c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                c_void_p]),
+    "fx_fp8_grouped_capacity": (c_int64, [c_int64, c_int]),
+    "fx_fp8_quantize_grouped_cols": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_int,
+                                             c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "fx_fp8_gemm_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "fx_fp8_gemm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64,
+                            c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+                            c_size_t, c_void_p]),
+    "fx_fp8_grouped_gemm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                    c_int64, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p,
+                                    c_int64, c_int, c_int, c_int, c_void_p]),
+    "fx_fp8_grouped_wgrad": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                     c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                     c_int, c_int, c_int, c_void_p]),
     "fx_swiglu_moe_bwd": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                   c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
                                   c_void_p]),
@@ -170,6 +202,33 @@ def stream_ptr(device=None) -> int:
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed (rc={rc}); see stderr for the reason")
+
+
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (a launch goes to the current device); free when it
+    already is."""
+    if t.device.type != "cuda" or t.device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(t.device)
+
+
+def require_same_device(*tensors: torch.Tensor, op: str) -> None:
+    """All given tensors on the GPU, and on one."""
+    require_gpu(*tensors, op=op)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{op}: tensors are on different devices: {sorted(map(str, devices))}")
 
 
 def require_gpu(*tensors: torch.Tensor, op: str) -> None:

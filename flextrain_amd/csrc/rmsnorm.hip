@@ -158,9 +158,10 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_generic_kernel(
 template <typename T, int LPR, int MAXV, int THREADS>
 __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
     const T* __restrict__ DY, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
-    const float* __restrict__ RSTD, T* __restrict__ DX, int accumulate_dx, T* __restrict__ YOUT,
+    const float* __restrict__ RSTD, T* DX, const T* OLD /* added to dx; may be DX; or null */, T* __restrict__ YOUT,
     float* __restrict__ PARTIAL /* [gridDim.x][ncols] or null */, int64_t rows, int ncols,
     int iters) {
+    const bool accumulate_dx = OLD != nullptr;
     constexpr int G = THREADS / LPR;
     extern __shared__ float smem[];  // [THREADS/64] reduction slots, then dW fold area
     float* red = smem;
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
                 for (int q = 0; q < PN; ++q) {
                     xr[v][q] = *reinterpret_cast<const Pack*>(X + row * ncols + col + q * VecOf<T>::N);
                     dyr[v][q] = *reinterpret_cast<const Pack*>(DY + row * ncols + col + q * VecOf<T>::N);
-                    if (accumulate_dx) oldr[v][q] = *reinterpret_cast<const Pack*>(DX + row * ncols + col + q * VecOf<T>::N);
+                    if (accumulate_dx) oldr[v][q] = *reinterpret_cast<const Pack*>(OLD + row * ncols + col + q * VecOf<T>::N);
                 }
             }
         }
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_reduce_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_generic_kernel(
     const T* __restrict__ DY, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
-    const float* __restrict__ RSTD, T* __restrict__ DX, int accumulate_dx, T* __restrict__ YOUT,
+    const float* __restrict__ RSTD, T* DX, const T* OLD /* added to dx; may be DX; or null */, T* __restrict__ YOUT,
     int64_t rows, int ncols) {
     __shared__ float red[4];
     __shared__ float s_k;
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_generic_kernel(
         const float xh = (float)x[c] * rstd;
         const float wv = wload(c);
         float dx = rstd * ((float)dy[c] * wv - xh * k);
-        if (accumulate_dx) dx = (float)DX[row * ncols + c] + dx;
+        if (OLD != nullptr) dx = (float)OLD[row * ncols + c] + dx;
         DX[row * ncols + c] = (T)dx;
         if (YOUT != nullptr) YOUT[row * ncols + c] = (T)(xh * wv);
     }
@@ -442,18 +443,19 @@ static int launch_fwd(const void* x, const void* w, int w_dt, void* y, float* rs
 
 template <typename T>
 static int launch_bwd(const void* dy, const void* x, const void* w, int w_dt, const float* rstd,
-                      void* dx, int acc_dx, void* yout, float* partial, int nblocks, int64_t rows,
+                      void* dx, const void* old, void* yout, float* partial, int nblocks, int64_t rows,
                       int ncols, const NormCfg& c, hipStream_t s) {
     const T* DY = reinterpret_cast<const T*>(dy);
     const T* X = reinterpret_cast<const T*>(x);
     T* DX = reinterpret_cast<T*>(dx);
+    const T* OLD = reinterpret_cast<const T*>(old);
     T* Y = reinterpret_cast<T*>(yout);
 #define FX_BWD_CASE(L, V, TH)                                                                     \
     if (c.lpr == L && c.maxv == V) {                                                              \
         constexpr int G = TH / L;                                                                 \
         const int iters = (int)((rows + (int64_t)nblocks * G - 1) / ((int64_t)nblocks * G));      \
         const size_t lds = sizeof(float) * (TH / 64 + (size_t)(G / 2) * L * V * 8);               \
-        rmsnorm_bwd_kernel<T, L, V, TH><<<nblocks, TH, lds, s>>>(DY, X, w, w_dt, rstd, DX, acc_dx, Y, partial, rows, ncols, iters); \
+        rmsnorm_bwd_kernel<T, L, V, TH><<<nblocks, TH, lds, s>>>(DY, X, w, w_dt, rstd, DX, OLD, Y, partial, rows, ncols, iters); \
         return 0;                                                                                 \
     }
     FX_BWD_CASE(16, 1, 1024) FX_BWD_CASE(32, 1, 1024) FX_BWD_CASE(64, 1, 1024) FX_BWD_CASE(64, 2, 512)
@@ -488,16 +490,16 @@ extern "C" size_t fx_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols) {
     return (size_t)bwd_grid(rows, groups) * (size_t)ncols * sizeof(float);
 }
 
-extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd,
-                              void* dx, int accumulate_dx, void* dw, int dw_dt, int accumulate_dw,
-                              void* y_out, int64_t rows, int ncols, int x_dt, int w_dt,
-                              float* ws, size_t ws_bytes, hipStream_t stream) {
+// dx = (old ? old : 0) + the norm's gradient; old may be dx itself or another buffer
+static int rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx, const void* old, void* dw,
+                       int dw_dt, int accumulate_dw, void* y_out, int64_t rows, int ncols, int x_dt, int w_dt, float* ws,
+                       size_t ws_bytes, hipStream_t stream) {
     if (rows < 0 || ncols <= 0) FX_FAIL("fx_rmsnorm_bwd: bad shape rows=%lld ncols=%d", (long long)rows, ncols);
     if (rows == 0) return 0;
     if (!dy || !x || !rstd || !dx) FX_FAIL("fx_rmsnorm_bwd: null pointer");
     const bool want_dw = (w != nullptr && dw != nullptr);
     NormCfg c;
-    bool vec = pick_cfg(ncols, c) && aligned16(dy) && aligned16(x) && aligned16(dx) &&
+    bool vec = pick_cfg(ncols, c) && aligned16(dy) && aligned16(x) && aligned16(dx) && (old == nullptr || aligned16(old)) &&
                (y_out == nullptr || aligned16(y_out)) && (w == nullptr || aligned16(w));
     if (vec && want_dw) {
         const size_t need = fx_rmsnorm_bwd_ws_bytes(rows, ncols);
@@ -508,7 +510,7 @@ extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, cons
         FX_DISPATCH_DTYPE(x_dt, T,
             rmsnorm_bwd_generic_kernel<T><<<dim3((unsigned)rows), 256, 0, stream>>>(
                 reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), w, w_dt, rstd,
-                reinterpret_cast<T*>(dx), accumulate_dx, reinterpret_cast<T*>(y_out), rows, ncols));
+                reinterpret_cast<T*>(dx), reinterpret_cast<const T*>(old), reinterpret_cast<T*>(y_out), rows, ncols));
         FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dx)");
         if (want_dw) {
             const unsigned grid = (unsigned)((ncols + 255) / 256);
@@ -525,7 +527,7 @@ extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, cons
     const int nblocks = bwd_grid(rows, groups);
     int rc = -1;
     FX_DISPATCH_DTYPE(x_dt, T,
-        rc = launch_bwd<T>(dy, x, w, w_dt, rstd, dx, accumulate_dx, y_out, want_dw ? ws : nullptr,
+        rc = launch_bwd<T>(dy, x, w, w_dt, rstd, dx, old, y_out, want_dw ? ws : nullptr,
                            nblocks, rows, ncols, c, stream));
     if (rc != 0) FX_FAIL("fx_rmsnorm_bwd: no kernel for ncols=%d", ncols);
     FX_CHECK_LAUNCH("fx_rmsnorm_bwd");
@@ -537,4 +539,18 @@ extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, cons
         FX_CHECK_LAUNCH("fx_rmsnorm_bwd(dw reduce)");
     }
     return 0;
+}
+
+extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd,
+                              void* dx, int accumulate_dx, void* dw, int dw_dt, int accumulate_dw,
+                              void* y_out, int64_t rows, int ncols, int x_dt, int w_dt,
+                              float* ws, size_t ws_bytes, hipStream_t stream) {
+    return rmsnorm_bwd(dy, x, w, rstd, dx, accumulate_dx ? dx : nullptr, dw, dw_dt, accumulate_dw, y_out, rows, ncols,
+                       x_dt, w_dt, ws, ws_bytes, stream);
+}
+
+extern "C" int fx_add_rmsnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx,
+                                  void* dw, int dw_dt, int accumulate_dw, int64_t rows, int ncols, int x_dt, int w_dt,
+                                  float* ws, size_t ws_bytes, hipStream_t stream) {
+    return rmsnorm_bwd(dy, h, w, rstd, dx, dh, dw, dw_dt, accumulate_dw, nullptr, rows, ncols, x_dt, w_dt, ws, ws_bytes, stream);
 }

@@ -3,6 +3,14 @@ ops on the per-layer training compute path, backed by libflexhip.so."""
 from __future__ import annotations
 
 from .adamw import flextrain_adamw_step
+from .fp8 import (
+    flextrain_fp8_grouped_matmul,
+    flextrain_fp8_grouped_wgrad,
+    flextrain_fp8_matmul,
+    flextrain_fp8_quantize,
+    flextrain_fp8_quantize_both,
+    flextrain_fp8_quantize_grouped_cols,
+)
 from .glu import (
     flextrain_gelu_tanh_gated_bwd,
     flextrain_gelu_tanh_gated_fwd,
@@ -25,6 +33,8 @@ from .moe import (
     flextrain_swiglu_moe_fwd,
 )
 from .rmsnorm import (
+    flextrain_add_rmsnorm_bwd,
+    flextrain_add_rmsnorm_fwd,
     flextrain_rmsnorm_bwd,
     flextrain_rmsnorm_fwd,
     flextrain_rmsnorm_fwd_recompute,
@@ -71,8 +81,16 @@ __all__ = [
     "flextrain_silu_bwd",
     "pin_tensor",
     "flextrain_adamw_step",
+    "flextrain_add_rmsnorm_bwd",
+    "flextrain_add_rmsnorm_fwd",
     "flextrain_copy_expert_counts",
     "flextrain_cross_entropy_loss",
+    "flextrain_fp8_grouped_matmul",
+    "flextrain_fp8_grouped_wgrad",
+    "flextrain_fp8_matmul",
+    "flextrain_fp8_quantize",
+    "flextrain_fp8_quantize_both",
+    "flextrain_fp8_quantize_grouped_cols",
     "flextrain_fused_topk_softmax",
     "flextrain_load_balance_bwd",
     "flextrain_moe_gather",

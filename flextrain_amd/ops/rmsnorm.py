@@ -9,7 +9,8 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import check, dtype_enum, lib, ptr, require_gpu, stream_ptr
+from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, require_gpu, require_same_device, stream_ptr
+from .fp8 import _fp8_rows, _round_up, _scale_store, _blocks
 
 
 def _norm_config(X, W, head_dim):
@@ -132,3 +133,78 @@ def flextrain_rmsnorm_bwd(dY, X, W, rstd, head_dim=None, dX=None, dW=None,
         stream_ptr(X.device))
     check(rc, "fx_rmsnorm_bwd")
     return dX, dw_buf, y_out
+
+
+def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_out=None, rms_norm_eps=1e-5):
+    """Residual addition and RMSNorm in one pass: ``(Y, scales, H, rstd)``.  The reference runs the addition, the norm
+    and any cast as separate passes; this op has no counterpart there.
+
+    ``H = X + residual`` rounded to ``X``'s dtype (``X`` itself without a residual), ``rstd (T, 1)`` fp32 of ``H``,
+    ``Y = H * rstd * W``.  ``output_dtype``: ``torch.float8_e4m3fn`` / ``torch.float8_e5m2`` give ``Y`` in 8 bits with
+    ``scales (T, ceil(D / 128))`` as :func:`flextrain_fp8_quantize` defines them (quantised from fp32: ``Y`` is not
+    rounded on the way); ``None`` gives ``Y`` in ``X``'s dtype, equal to ``flextrain_rmsnorm_fwd(H, W)``, and no
+    scales.  ``sum_out`` receives ``H`` and may be ``X`` or ``residual``."""
+    op = "flextrain_add_rmsnorm_fwd"
+    T, D, _, _ = _norm_config(X, W, None)
+    if D == 0:
+        raise ValueError(f"{op}: X has no columns")
+    for t, name in ((residual, "residual"), (sum_out, "sum_out")):
+        if t is not None:
+            _check_like(t, X, name)
+    require_same_device(X, residual, W, sum_out, op=op)
+    x_dt = dtype_enum(X.dtype)
+    y_dt = x_dt if output_dtype is None or output_dtype == X.dtype else fp8_enum(output_dtype)
+    H = sum_out
+    if H is None:
+        H = torch.empty_like(X) if residual is not None else X
+    rstd = torch.empty(T, 1, dtype=torch.float32, device=X.device)
+    if y_dt == x_dt:
+        Y, scales, ldy = torch.empty_like(X), None, D
+    else:
+        Y, scales, ldy = _fp8_rows((), T, D, output_dtype, X.device), _scale_store((), T, _blocks(D), X.device), _round_up(D, 16)
+    with on_device(X):
+        rc = lib().fx_add_rmsnorm_fwd(ptr(X), ptr(residual), ptr(W), ptr(H) if H is not X or residual is not None else None,
+                                      ptr(Y), ldy, ptr(scales), T, ptr(rstd), T, D, float(rms_norm_eps), x_dt,
+                                      dtype_enum(W.dtype) if W is not None else 0, y_dt, stream_ptr(X.device))
+    check(rc, "fx_add_rmsnorm_fwd")
+    return Y, scales, H, rstd
+
+
+def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
+    """``(dX, dW)`` of :func:`flextrain_add_rmsnorm_fwd`: ``dX = dH + (gradient of the norm)`` is the gradient of ``X``
+    and of ``residual`` alike.
+
+    ``dH`` is the gradient that reaches ``H`` past the norm (the residual stream's; ``None``: zero) and is left as it is
+    unless it is given as ``dX`` too.  ``dY`` is the gradient of the unquantised output (the 8-bit rounding is passed
+    straight through).  ``dW``: accumulated into when given, else a fresh fp32 gradient; ``None`` without ``W``."""
+    op = "flextrain_add_rmsnorm_bwd"
+    T, D, _, _ = _norm_config(H, W, None)
+    for t, name in ((dY, "dY"), (dH, "dH"), (dX, "dX")):
+        if t is not None:
+            _check_like(t, H, name)
+    if rstd.numel() != T or not rstd.is_contiguous() or rstd.dtype != torch.float32:
+        raise ValueError(f"rstd must be a contiguous float32 tensor of shape {(T, 1)}")
+    if W is None and dW is not None:
+        raise ValueError(f"{op}: dW without W")
+    if dW is not None and (tuple(dW.shape) != (D,) or not dW.is_contiguous()):
+        raise ValueError(f"dW must be contiguous of shape {(D,)}")
+    require_same_device(dY, H, W, rstd, dH, dX, dW, op=op)
+    if dX is None:
+        dX = torch.empty_like(H)
+    accumulate = dW is not None
+    if W is not None and dW is None:
+        dW = torch.empty(D, dtype=torch.float32, device=H.device)
+        if T == 0:
+            dW.zero_()
+    if T == 0:
+        return dX, dW
+    L = lib()
+    with on_device(H):
+        nbytes = int(L.fx_rmsnorm_bwd_ws_bytes(T, D)) if dW is not None else 0
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=H.device) if nbytes else None
+        rc = L.fx_add_rmsnorm_bwd(ptr(dY), ptr(dH), ptr(H), ptr(W), ptr(rstd), ptr(dX), ptr(dW),
+                                  dtype_enum(dW.dtype) if dW is not None else 0, 1 if accumulate else 0, T, D,
+                                  dtype_enum(H.dtype), dtype_enum(W.dtype) if W is not None else 0, ptr(ws), nbytes,
+                                  stream_ptr(H.device))
+    check(rc, "fx_add_rmsnorm_bwd")
+    return dX, dW

@@ -34,6 +34,11 @@ typedef struct ihipStream_t* hipStream_t;
 #define FX_DT_F16 1
 #define FX_DT_BF16 2
 
+/* 8-bit floating point (OCP e4m3, largest 448; e5m2, largest 57344), held with one power-of-two scale
+ * per block of 128 values: the byte e + 127 stands for 2^e (e8m0). */
+#define FX_DT_E4M3 3
+#define FX_DT_E5M2 4
+
 #define FX_ACT_SILU 0
 #define FX_ACT_GELU_TANH 1
 
@@ -490,6 +495,80 @@ double solve_scheduler(int T, int N, int k, const double* compute, const double*
  * for solve_scheduler, a power of two >= 2048. */
 int compute_buf_size(int T, int N, int k, const double* compute, const double* durations, double deadline,
                      int time_scale);
+
+/* ---- 8-bit path (no counterpart in the reference, whose kernels are 16-bit and wider) ------------- */
+
+/* h = x + residual rounded to x's dtype; rstd = (mean(h^2) + eps)^-1/2; y = h * rstd * w.
+ * x, residual, h: (rows, ncols) contiguous, dtype x_dt; residual may be NULL (then h = x, and h may be
+ * NULL); h may be x or residual.  w: (ncols,) of dtype w_dt or NULL.  rstd: fp32 (rows,).
+ * y_dt == x_dt: y (rows, ncols) contiguous, rounded as fx_rmsnorm_fwd rounds; s is not used.
+ * y_dt FX_DT_E4M3 / FX_DT_E5M2: y holds 8-bit rows ldy apart (ldy = ncols rounded up to 16, the bytes in
+ * between are written as 0), s the scale bytes, of row r and columns [128 b, 128 b + 128) at s[b * lds + r]. */
+int fx_add_rmsnorm_fwd(const void* x, const void* residual, const void* w, void* h, void* y, int64_t ldy, void* s,
+                       int64_t lds, float* rstd, int64_t rows, int ncols, float eps, int x_dt, int w_dt, int y_dt,
+                       hipStream_t stream);
+
+/* Gradient of x and residual alike: dx = (dh ? dh : 0) + the norm's gradient of dy, dh being the gradient that
+ * reaches h past the norm (dx may be dh).  dw (ncols,) of dtype dw_dt or NULL; workspace and accumulate_dw as
+ * in fx_rmsnorm_bwd. */
+int fx_add_rmsnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx,
+                       void* dw, int dw_dt, int accumulate_dw, int64_t rows, int ncols, int x_dt, int w_dt,
+                       float* ws, size_t ws_bytes, hipStream_t stream);
+
+/* x (rows, cols), row stride ldx, any of fp32 / fp16 / bf16, to 8-bit values with block scales: 2^e with the
+ * smallest e that brings the block's largest finite magnitude to at most the type's largest number, e = 0 for
+ * a block of zeros; infinities and NaN stay what they are (e4m3: NaN).
+ *   tiles == 0: q (rows, ldq), block 1 x 128, scale of (r, column block b) at s[b * lds + r];  with qt:
+ *               qt (cols, ldt) the transposed matrix, block 128 rows x 1 column, scale of (column c, row block
+ *               b) at st[b * ldst + c]
+ *   tiles != 0: block 128 x 128, scale of (row block i, column block b) at s[b * lds + i], and for qt the same
+ *               scales at st[i * ldst + b]
+ * ldq / ldt: cols / rows rounded up to 16; the bytes in between are written as 0.  qt and st NULL: not made.
+ * batch matrices of that shape, the *_batch arguments (elements) apart (the weights of all experts at once). */
+int fx_fp8_quantize(const void* x, int64_t ldx, int64_t x_batch, int batch, int64_t rows, int64_t cols, int x_dt,
+                    int q_dt, int tiles, void* q, int64_t ldq, int64_t q_batch, void* s, int64_t lds, int64_t s_batch,
+                    void* qt, int64_t ldt, int64_t qt_batch, void* st, int64_t ldst, int64_t st_batch,
+                    hipStream_t stream);
+
+/* Row capacity of the expert-padded order: room for every split of `rows` rows over E experts when each
+ * expert's rows start at a multiple of 128. */
+int64_t fx_fp8_grouped_capacity(int64_t rows, int E);
+
+/* Expert-sorted rows (counts[e] consecutive rows of expert e; counts on the device) to the transposed 8-bit
+ * matrix qt (cols, ldt = fx_fp8_grouped_capacity(rows, E)) in which every expert's rows start at a multiple of
+ * 128, with scales per 128 rows of one column at st[b * ldst + c]; places without a row hold 0 with scale 1.
+ * row_map (or NULL): sorted row r is row row_map[r] of x, which then has src_rows rows (entries are clamped to
+ * them).  At most 2^24 rows. */
+int fx_fp8_quantize_grouped_cols(const void* x, int64_t ldx, int64_t src_rows, int64_t rows, int64_t cols, int x_dt,
+                                 int q_dt, const int32_t* counts, int E, const int32_t* row_map, void* qt, int64_t ldt,
+                                 void* st, int64_t ldst, hipStream_t stream);
+
+/* D (M, N) = A (M, K) B (N, K)^T + C, accumulated in fp32.  A: a_dt e4m3 or e5m2, B e4m3; rows start at 16-byte
+ * addresses.  The scale of row r and k block b is SA[(a_tiles ? r / 128 : r) * sa_row + b * sa_k], SB likewise.
+ * C (or NULL) and D: dtype d_dt (0 / 1 / 2); C may be D.  ws: fx_fp8_gemm_ws_bytes bytes, 16-byte aligned (may be
+ * NULL when that is 0); calls that may overlap need one each. */
+size_t fx_fp8_gemm_ws_bytes(int M, int N, int K);
+int fx_fp8_gemm(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k, int a_tiles,
+                const void* B, int64_t ldb, const void* SB, int64_t sb_row, int64_t sb_k, int b_tiles, const void* C,
+                int64_t ldc, void* D, int64_t ldd, int M, int N, int K, int d_dt, void* ws, size_t ws_bytes,
+                hipStream_t stream);
+
+/* D[rows of e] = A[rows of e] B[e]^T for every expert, one launch; counts (E) on the device.  B[e] is (N, K) at
+ * B + e * b_expert, its scales at SB + e * sb_expert.  row_map (or NULL): expert-sorted row r is row row_map[r]
+ * of A (a_rows rows; entries are clamped to them).  Rows of D behind the last expert's stay as they were. */
+int fx_fp8_grouped_gemm(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k,
+                        const int32_t* row_map, int64_t a_rows, const void* B, int64_t ldb, int64_t b_expert,
+                        const void* SB, int64_t sb_row, int64_t sb_k, int64_t sb_expert, int b_tiles,
+                        const int32_t* counts, int E, int64_t total_rows, void* D, int64_t ldd, int N, int K, int d_dt,
+                        hipStream_t stream);
+
+/* D[e] (M, N) = A_e B_e^T + C[e], A_e / B_e the columns of expert e of A (M, capacity) / B (N, capacity) in the
+ * expert-padded order fx_fp8_quantize_grouped_cols writes.  An expert without rows gives C[e] (or 0). */
+int fx_fp8_grouped_wgrad(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k,
+                         const void* B, int64_t ldb, const void* SB, int64_t sb_row, int64_t sb_k,
+                         const int32_t* counts, int E, int64_t capacity, const void* C, int64_t ldc,
+                         int64_t c_expert, void* D, int64_t ldd, int64_t d_expert, int M, int N, int d_dt,
+                         hipStream_t stream);
 
 #ifdef __cplusplus
 }

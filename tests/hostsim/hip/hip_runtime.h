@@ -156,6 +156,17 @@ inline int __any(int pred) {
     hostsim::sync_wave();
     return any;
 }
+inline unsigned long long __ballot(int pred) {
+    const unsigned me = hostsim::flat_thread(), wave0 = me & ~63u;
+    const unsigned lanes = hostsim::g_block_dim.x * hostsim::g_block_dim.y * hostsim::g_block_dim.z;
+    hostsim::g_exchange[me] = pred != 0;
+    hostsim::sync_wave();
+    unsigned long long who = 0;
+    for (unsigned l = wave0; l < wave0 + 64 && l < lanes; ++l)
+        if (hostsim::g_alive[l] && hostsim::g_exchange[l] != 0) who |= 1ull << (l - wave0);
+    hostsim::sync_wave();
+    return who;
+}
 template <typename T> inline T atomicAdd(T* p, T v) { T old = *p; *p = old + v; return old; }      // fibers never preempt each other
 template <typename T> inline T atomicOr(T* p, T v) { T old = *p; *p = old | v; return old; }
 template <typename T> inline T atomicMax(T* p, T v) { T old = *p; *p = std::max(old, v); return old; }
@@ -215,6 +226,65 @@ inline Acc mfma32x32x16(Frag a, Frag b, Acc c) {
     return c;
 }
 
+// 8-bit floating point: e4m3 (bias 7, no infinity, S.1111.111 is NaN) and e5m2 (bias 15, IEEE-like).
+inline float fp8_value(unsigned char b, bool e5m2) {
+    const int mbits = e5m2 ? 2 : 3, bias = e5m2 ? 15 : 7;
+    const int mant = b & ((1 << mbits) - 1), ex = (b >> mbits) & (e5m2 ? 31 : 15);
+    float v;
+    if (e5m2 && ex == 31) v = mant ? NAN : INFINITY;
+    else if (!e5m2 && ex == 15 && mant == 7) v = NAN;
+    else v = ex ? ldexpf((float)(mant + (1 << mbits)), ex - bias - mbits) : ldexpf((float)mant, 1 - bias - mbits);
+    return b & 0x80 ? -v : v;
+}
+// nearest even; finite values past the largest number become NaN (e4m3) or infinity (e5m2)
+inline unsigned char fp8_code(float x, bool e5m2) {
+    const int mbits = e5m2 ? 2 : 3, low = e5m2 ? -14 : -6;
+    const unsigned char sign = std::signbit(x) ? 0x80 : 0, top = e5m2 ? 0x7b : 0x7e;
+    if (std::isnan(x)) return sign | 0x7f;
+    const float a = fabsf(x);
+    if (std::isinf(a)) return sign | (e5m2 ? 0x7c : 0x7f);
+    if (a == 0.f) return sign;
+    int p;
+    frexpf(a, &p);
+    const int ex = std::max(p - 1, low);
+    const double steps = nearbyint(ldexp((double)a, mbits - ex));       // of 2^(ex - mbits)
+    const int code = (int)steps + ((ex - low) << mbits);                // the codes are consecutive across binades
+    return sign | (unsigned char)(code > top ? (e5m2 ? 0x7c : 0x7f) : code);
+}
+inline int cvt_pk_8(float a, float b, int old, bool high, bool e5m2) {
+    const unsigned two = fp8_code(a, e5m2) | ((unsigned)fp8_code(b, e5m2) << 8);
+    return high ? (int)(((unsigned)old & 0xffffu) | (two << 16)) : (int)(((unsigned)old & 0xffff0000u) | two);
+}
+
+// v_mfma_scale_f32_32x32x64_f8f6f4 with 8-bit operands: D = A (32 x 64) * B (64 x 32) + C, every 32 k of an
+// operand row times 2^(byte - 127) (byte 255: NaN).  Lane l supplies A[l % 32][32 (l / 32) .. + 31], B likewise,
+// and the scale bytes of those values; the accumulator layout is that of the 16-bit instruction.
+// The 16x16x128 form: lane l supplies row l % 16, k 32 (l / 16) .. + 31; register v of lane l is
+// D[4 (l / 16) + v][l % 16].
+extern float (*g_wave_f8)[64][64];              // [wave][lane][32 of A, 32 of B], scaled
+template <int N, typename Frag, typename Acc>
+inline Acc mfma_scale(Frag a, Frag b, Acc c, int fmt_a, int fmt_b, int opsel_a, int scale_a, int opsel_b, int scale_b) {
+    constexpr int K_LANES = 64 / N;             // lanes that share a row
+    const unsigned me = flat_thread(), w = me >> 6, l = me & 63u;
+    float* mine = g_wave_f8[w][l];
+    const unsigned char *pa = reinterpret_cast<const unsigned char*>(&a), *pb = reinterpret_cast<const unsigned char*>(&b);
+    const int ba = (scale_a >> (8 * opsel_a)) & 255, bb = (scale_b >> (8 * opsel_b)) & 255;
+    const float sa = ba == 255 ? NAN : ldexpf(1.f, ba - 127), sb = bb == 255 ? NAN : ldexpf(1.f, bb - 127);
+    for (int j = 0; j < 32; ++j) { mine[j] = fp8_value(pa[j], fmt_a == 1) * sa; mine[32 + j] = fp8_value(pb[j], fmt_b == 1) * sb; }
+    sync_wave();
+    for (int v = 0; v < N * N / 64; ++v) {
+        const unsigned row = N == 32 ? 8u * (v / 4) + 4u * (l / 32) + (unsigned)(v % 4) : 4u * (l / 16) + (unsigned)v;
+        float sum = c[v];
+        for (int q = 0; q < K_LANES; ++q) {
+            const float *x = g_wave_f8[w][row + N * q], *y = g_wave_f8[w][l % N + N * q] + 32;
+            for (int k = 0; k < 32; ++k) sum += x[k] * y[k];
+        }
+        c[v] = sum;
+    }
+    sync_wave();
+    return c;
+}
+
 // ds_read_b64_tr_b16: inside each group of 16 lanes, lane s receives, for j = 0 .. 3, element s % 4 of the
 // 8 bytes that lane 4 j + s / 4 of the group addressed.
 template <typename V4>
@@ -242,6 +312,10 @@ inline unsigned perm_b32(unsigned hi, unsigned lo, unsigned sel) {
 
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) hostsim::mfma32x32x16(a, b, c)
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) hostsim::mfma32x32x16(a, b, c)
+#define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<32>(a, b, c, fa, fb, oa, sa, ob, sb)
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<16>(a, b, c, fa, fb, oa, sa, ob, sb)
+#define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, false)
+#define __builtin_amdgcn_cvt_pk_bf8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, true)
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) hostsim::ds_read_tr16<short __attribute__((ext_vector_type(4)))>((const void*)(p))
 #define __builtin_amdgcn_perm(hi, lo, sel) hostsim::perm_b32(hi, lo, sel)
 

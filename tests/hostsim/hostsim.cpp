@@ -33,6 +33,8 @@ static unsigned char* const g_lds_region = map_lds();
 unsigned char* g_dynamic_lds = g_lds_region;
 static float g_wave_store[MAX_LANES / 64][64][16];
 float (*g_wave_f32)[64][16] = g_wave_store;
+static float g_wave_f8_store[MAX_LANES / 64][64][64];
+float (*g_wave_f8)[64][64] = g_wave_f8_store;
 
 // Fiber switch: the callee-saved registers go on the old stack, the stack pointers are exchanged
 // (swapcontext would make a signal-mask system call per switch, and a GEMM tile makes millions).
