@@ -79,54 +79,84 @@ FX_DEV void load8_or_zero(const T* row, int64_t col, int64_t cols, float (&o)[8]
 
 // ---------------------------------------------------------------- experts
 // Expert-sorted rows: expert e owns COUNTS[e] consecutive rows.  The counts stay on the device, so a workgroup
-// finds its place itself: the 64 lanes of a wave look at 64 experts at a time (two scans over the lanes).  The
-// counts may promise more rows than there are (the host cannot check them): a count is cut to the rows that
-// are left, so no address leaves the buffers.  total_rows is at most 2^24, 64 counts fit 32 bits.
-struct GroupTile {
+// finds its place itself: the 64 lanes of a wave look at 64 experts at a time (a scan over the lanes for the rows, one
+// for the tiles).  The counts may promise more rows than there are (the host cannot check them): a count is cut to
+// the rows that are left, so every tile that exists has rows and no address leaves the buffers.  total_rows is at
+// most 2^24, 64 counts fit 32 bits.
+
+// A value that all lanes hold alike, in a scalar register.
+FX_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+FX_DEV int wave_scan(int v, int lane) {          // inclusive
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int a = __shfl_up(v, off, 64);
+        if (lane >= off) v += a;
+    }
+    return v;
+}
+
+// Expert e0 + lane of a step over 64 experts: its first row and its rows (cut to what is left), given the rows before
+// the step; moves row_base behind the step.
+FX_DEV void group_rows(const int32_t* COUNTS, int E, int e0, int total_rows, int lane, int& row_base, int& row0, int& rows) {
+    const int c = e0 + lane < E ? min(max(COUNTS[e0 + lane], 0), total_rows) : 0;
+    const int sum = wave_scan(c, lane);
+    row0 = min(row_base + sum - c, total_rows);
+    rows = min(c, total_rows - row0);
+    row_base = min(row_base + uniform(__shfl(sum, 63, 64)), total_rows);
+}
+
+struct GroupTile {     // (the same in every lane, and held in scalar registers)
     int e;             // expert, -1: the tile belongs to none
-    int64_t row0;      // its first row
+    int row0;          // its first row
     int rows;          // its rows
-    int m0;            // first row of the tile within the expert
+    int m0;            // first row of the tile within the expert, below `rows`
 };
 
 // Tile `tile` of the list of all experts' tiles of 2^SHIFT rows (an expert without rows has no tile).
 template <int SHIFT>
-FX_DEV GroupTile find_group_tile(const int32_t* COUNTS, int E, int64_t tile, int64_t total_rows, int lane) {
-    int64_t row_base = 0, tile_base = 0;
+FX_DEV GroupTile find_group_tile(const int32_t* COUNTS, int E, int tile, int64_t total_rows, int lane) {
+    int row_base = 0, tile_base = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
-        const int e = e0 + lane;
-        const int c = e < E ? min(max(COUNTS[e], 0), (int)total_rows) : 0;
-        const int nt = (c + (1 << SHIFT) - 1) >> SHIFT;
-        int ir = c, it = nt;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int a = __shfl_up(ir, off, 64), b = __shfl_up(it, off, 64);
-            if (lane >= off) { ir += a; it += b; }
-        }
-        const bool mine = tile >= tile_base + it - nt && tile < tile_base + it;
-        const unsigned long long who = __ballot(mine);
+        int row0, rows;
+        group_rows(COUNTS, E, e0, (int)total_rows, lane, row_base, row0, rows);
+        const int nt = (rows + (1 << SHIFT) - 1) >> SHIFT;
+        const int it = tile_base + wave_scan(nt, lane);
+        const unsigned long long who = __ballot(tile >= it - nt && tile < it);
         if (who != 0ull) {
             const int src = (int)__builtin_ctzll(who);
             GroupTile t;
-            t.e = e0 + src;
-            t.row0 = row_base + __shfl(ir - c, src, 64);
-            t.rows = (int)min((int64_t)__shfl(c, src, 64), max((int64_t)0, total_rows - t.row0));
-            t.m0 = (int)(tile - tile_base - __shfl(it - nt, src, 64)) << SHIFT;
+            t.e = uniform(e0 + src);
+            t.row0 = uniform(__shfl(row0, src, 64));
+            t.rows = uniform(__shfl(rows, src, 64));
+            t.m0 = uniform((tile - __shfl(it - nt, src, 64)) << SHIFT);
             return t;
         }
-        row_base += __shfl(ir, 63, 64);
-        tile_base += __shfl(it, 63, 64);
+        tile_base = uniform(__shfl(it, 63, 64));
     }
     return GroupTile{-1, 0, 0, 0};
 }
 
+// Number of such tiles.
+template <int SHIFT>
+FX_DEV int count_group_tiles(const int32_t* COUNTS, int E, int64_t total_rows, int lane) {
+    int n = 0, row_base = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        int row0, rows;
+        group_rows(COUNTS, E, e0, (int)total_rows, lane, row_base, row0, rows);
+        n += (rows + (1 << SHIFT) - 1) >> SHIFT;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+    return uniform(n);
+}
+
 // Rows of expert e, and where they start when every expert's rows begin at a multiple of 128.
 struct GroupSpan {
-    int64_t padded0;
-    int rows;
+    int padded0, rows;
 };
 FX_DEV GroupSpan find_group_span(const int32_t* COUNTS, int E, int e, int64_t capacity, int lane) {
-    int64_t padded0 = 0;
+    int padded0 = 0;
     int mine = 0;
     for (int e0 = 0; e0 <= e; e0 += 64) {
         const int i = e0 + lane;
@@ -134,12 +164,12 @@ FX_DEV GroupSpan find_group_span(const int32_t* COUNTS, int E, int e, int64_t ca
         int p = i < e ? (c + 127) & ~127 : 0;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) p += __shfl_xor(p, off, 64);
-        padded0 += p;
-        if (e < e0 + 64) mine = __shfl(c, e - e0, 64);
+        padded0 = min(padded0 + uniform(p), (int)capacity);
+        if (e < e0 + 64) mine = uniform(__shfl(c, e - e0, 64));
     }
     GroupSpan s;
     s.padded0 = padded0;
-    s.rows = padded0 + ((mine + 127) & ~127) <= capacity ? mine : 0;
+    s.rows = padded0 + ((mine + 127) & ~127) <= (int)capacity ? mine : 0;
     return s;
 }
 

@@ -1,0 +1,393 @@
+// Tile code of the 8-bit products (see fp8_gemm.hip for what they compute), gfx950.
+//
+// A workgroup of WAVES_M x WAVES_N waves owns a BM x BN tile of D and walks K in steps of 128 bytes, one scale
+// block.  Both operands go from memory straight into LDS (global_load_lds_dwordx4), two LDS stages alternate, one
+// barrier per K-step.  LDS row r holds its 128 k-values as eight 16-byte chunks, chunk c at position
+// c ^ ((r >> 1) & 7): 16 lanes of a fragment read (16 consecutive rows, one chunk) then touch all 64 banks once.
+// The matrix instruction takes 32 consecutive k of a row per lane: two 16-byte LDS reads a fragment.  It runs for
+// 64 cycles, twice as long as the 16-bit one on the same number of bytes, so a K-step costs the matrix pipe and the
+// LDS exactly what a 64-wide K-step of the 16-bit core costs them, for twice the arithmetic.
+#pragma once
+#include "fp8.h"
+#include "gemm_core2.h"
+
+namespace fx {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int FP8_BK = 128;
+
+// A wave-uniform pointer to global memory held in scalar registers (a no-op where the compiler knows).
+typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
+FX_DEV global_bytes uniform_ptr(const uint8_t* p) {
+    const uint64_t u = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<global_bytes>(((uint64_t)(unsigned)uniform((int)(u >> 32)) << 32) | (uint64_t)(unsigned)uniform((int)(unsigned)u));
+}
+
+// One operand: rows of 8-bit values, and the scale of (row, k block) at s[(row >> s_shift) * s_row + kb * s_k].
+// A scale tensor spans less than 2^31 bytes, a row 2^23 (the host checks): lane offsets are 32 bits wide.
+struct Fp8View {
+    const uint8_t* p;
+    const uint8_t* s;
+    int ld, s_row, s_k;
+    int s_shift;      // 0: a scale per row, 7: per 128 rows
+    int ext;          // rows
+};
+
+// What a workgroup does next: D rows [m0, m0 + BM), columns [n0, n0 + BN) of one product.
+template <typename TD>
+struct Fp8Job {
+    Fp8View A, B;
+    int m0, n0, K;
+    const int32_t* row_map;       // A row r of this product is source row row_map[r] (A.p, A.s: the whole source), or null
+    int src_rows;
+    const TD* C;
+    TD* D;
+};
+
+// The B fragment goes first: the accumulator then holds the transposed tile, a lane four consecutive columns of D.
+// SB / SA: which byte of the packed scales belongs to the fragment.
+template <int AF, int SB, int SA>
+FX_DEV f32x16_t mfma_fp8(const i32x8_t& b, const i32x8_t& a, f32x16_t c, int sb, int sa) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, c, 0, AF == DT_E4M3 ? 0 : 1, SB, sb, SA, sa);
+}
+
+// 16 k-values of a row from k on, 0 behind K.  Rows start at 16-byte addresses; a chunk that K ends inside is read
+// byte by byte (what lies behind K in memory is not the operand's).
+FX_DEV u32x4_t load_chunk(const uint8_t* row, int k, int K) {
+    union { u32x4_t q; uint8_t b[16]; } u;
+    if (k + 16 <= K) return ldg16(row + k);
+    const u32x4_t zero = {0u, 0u, 0u, 0u};
+    u.q = zero;
+    for (int j = 0; j < 16; ++j)
+        if (k + j < K) u.b[j] = row[k + j];
+    return u.q;
+}
+
+template <int AF, typename TD, int BM, int BN, int WAVES_M, int WAVES_N>
+struct Fp8Loop {
+    static constexpr int NW = WAVES_M * WAVES_N, NT = NW * 64;
+    static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
+    static constexpr int TM = WM / 32, TN = WN / 32, MFMAS = TM * TN;
+    static constexpr int NA = BM / 8 / NW, NB = BN / 8 / NW, LD = NA + NB;      // 1 KB load instructions per wave and K-step
+    static constexpr int STAGE = (BM + BN) * FP8_BK;                            // bytes
+    static constexpr int HI = TM / 2;                                           // A fragments with two register sets
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile rows must split evenly over the waves");
+    static_assert(TM >= 2 && TM % 2 == 0 && TM <= 4 && TN == 2, "fragment schedule below");
+    static constexpr int PER = (LD + MFMAS - 1) / MFMAS;
+
+    // fragments: a sub-step (64 k) needs TM of A and TN of B.  B and the upper half of A have two register sets that
+    // alternate between the two sub-steps of a K-step; the lower half of A is read again as soon as its last MFMA
+    // is issued.  All reads of a sub-step are then out two MFMAs before its end.
+    i32x8_t alo[TM - HI], ahi[2][HI], bf[2][TN];
+    unsigned aoff[NA], boff[NB];          // lane byte offsets of the tile loads
+    const uint8_t *abase, *bbase;
+    unsigned soa[TM / 2], sob;            // lane offsets of the scales: lane l fetches rows l, 64 + l, .. of its wave's
+    const uint8_t *sabase, *sbbase;
+    int sak, sbk;
+    int rawa[TM / 2], rawb;               // scale bytes requested for the next K-step
+    int sca, scb;                         // packed scales of the current one
+    int wave, lane;
+
+    // source row of tile row r of A (clamped to the last one; its products are never stored)
+    static FX_DEV int64_t a_row(const Fp8Job<TD>& j, int r) {
+        const int g = min(j.m0 + r, j.A.ext - 1);
+        // a map entry outside the source must not turn into an address outside it
+        return j.row_map != nullptr ? (int64_t)min(max(j.row_map[g], 0), j.src_rows - 1) : (int64_t)g;
+    }
+
+    // one instruction of a K-step's loads
+    template <int IDX>
+    FX_DEV void issue_one(uint8_t* buf) {
+        if constexpr (IDX < NA) {
+            load_to_lds16_s(aoff[IDX], abase, (unsigned)(uintptr_t)(buf + (IDX * NW + wave) * 1024));
+            if (IDX == NA - 1) abase += FP8_BK;
+        } else if constexpr (IDX < LD) {
+            load_to_lds16_s(boff[IDX - NA], bbase, (unsigned)(uintptr_t)(buf + BM * FP8_BK + ((IDX - NA) * NW + wave) * 1024));
+            if (IDX == LD - 1) bbase += FP8_BK;
+        }
+    }
+    FX_DEV void issue(uint8_t* buf) { static_for<0, LD>([&](auto i) { issue_one<decltype(i)::value>(buf); }); }
+
+    FX_DEV void fetch_scales() {
+#pragma unroll
+        for (int i = 0; i < TM / 2; ++i) rawa[i] = uniform_ptr(sabase)[soa[i]];
+        rawb = uniform_ptr(sbbase)[sob];
+        sabase += sak;
+        sbbase += sbk;
+    }
+    // Byte i of the packed scales belongs to fragment i, whose row in lane l is 32 i + l % 32; lane l has fetched the
+    // bytes of rows 64 u + l.  Exchanging the upper half of one copy with the lower half of another leaves the bytes of
+    // rows 64 u + l % 32 in the first and those of rows 64 u + 32 + l % 32 in the second.
+    FX_DEV void pack_scales(int& a, int& b) const {
+        unsigned w = (unsigned)rawa[0];
+        if constexpr (TM == 4) w |= (unsigned)rawa[1] << 16;
+        const auto x = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        a = (int)(x[0] | (x[1] << 8));
+        const auto y = __builtin_amdgcn_permlane32_swap((unsigned)rawb, (unsigned)rawb, false, false);
+        b = (int)(y[0] | (y[1] << 8));
+    }
+
+    // Set up the tile and request its first K-step into buf0.
+    FX_DEV void begin(const Fp8Job<TD>& j, uint8_t* buf0) {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+        const int rr = lane >> 3, pos = lane & 7;
+        const bool gathered = j.row_map != nullptr;
+        // offsets are taken from the tile's first row (gathered: from the source's, which is below 4 GB)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int r = (i * NW + wave) * 8 + rr;
+            const int64_t row = a_row(j, r) - (gathered ? 0 : j.m0);
+            aoff[i] = (unsigned)(row * j.A.ld + ((pos ^ swz(r)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int r = (i * NW + wave) * 8 + rr;
+            boff[i] = (unsigned)((int64_t)(min(j.n0 + r, j.B.ext - 1) - j.n0) * j.B.ld + ((pos ^ swz(r)) << 4));
+        }
+        abase = j.A.p + (gathered ? 0 : (int64_t)j.m0 * j.A.ld);
+        bbase = j.B.p + (int64_t)j.n0 * j.B.ld;
+#pragma unroll
+        for (int i = 0; i < TM / 2; ++i) soa[i] = (unsigned)((int)a_row(j, wm * WM + i * 64 + lane) >> j.A.s_shift) * (unsigned)j.A.s_row;
+        sob = (unsigned)(min(j.n0 + wn * WN + lane, j.B.ext - 1) >> j.B.s_shift) * (unsigned)j.B.s_row;
+        sabase = j.A.s;
+        sbbase = j.B.s;
+        sak = j.A.s_k;
+        sbk = j.B.s_k;
+        if (j.K >= FP8_BK) issue(buf0);
+        if (j.K > 0) fetch_scales();
+    }
+
+    // The 32 k-values of this lane in tile row row0 + (lane & 31), sub-step ks.
+    FX_DEV i32x8_t read_frag(const uint8_t* tile, int row0, int ks) const {
+        const int r = lane & 31, h = lane >> 5, s = swz(r);        // row0 is a multiple of 32: swz(row0 + r) = swz(r)
+        const uint8_t* p = tile + (row0 + r) * FP8_BK;
+        const int c = ks * 4 + h * 2;
+        union { i32x8_t f; u32x4_t q[2]; } u;
+        u.q[0] = *reinterpret_cast<const u32x4_t*>(p + ((c ^ s) << 4));
+        u.q[1] = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ s) << 4));
+        return u.f;
+    }
+    template <int I, int P>
+    FX_DEV void read_a(const uint8_t* buf, int ks) {
+        const int row0 = (wave / WAVES_N) * WM + I * 32;
+        if constexpr (I < TM - HI) alo[I] = read_frag(buf, row0, ks);
+        else ahi[P][I - (TM - HI)] = read_frag(buf, row0, ks);
+    }
+    template <int J, int P>
+    FX_DEV void read_b(const uint8_t* buf, int ks) {
+        bf[P][J] = read_frag(buf + BM * FP8_BK, (wave % WAVES_N) * WN + J * 32, ks);
+    }
+
+    // MFMAs of the sub-step whose fragments are in register set P; with FETCH the fragments of sub-step ks_f in `buf`
+    // are read into set 1 - P meanwhile.  after(IntC<M>) runs in the shadow of MFMA M.
+    template <int P, bool FETCH, int M = 0, typename After>
+    FX_DEV void sub(f32x16_t (&acc)[TM][TN], const uint8_t* buf, int ks_f, After&& after) {
+        if constexpr (M < MFMAS) {
+            constexpr int i = M / TN, j = M % TN, Q = 1 - P;
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (i < TM - HI) acc[i][j] = mfma_fp8<AF, j, i>(bf[P][j], alo[i], acc[i][j], scb, sca);
+            else acc[i][j] = mfma_fp8<AF, j, i>(bf[P][j], ahi[P][i - (TM - HI)], acc[i][j], scb, sca);
+            if constexpr (FETCH) {
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (TM == 4) {
+                    if constexpr (M == 0) read_b<0, Q>(buf, ks_f);
+                    if constexpr (M == 1) read_b<1, Q>(buf, ks_f);
+                    if constexpr (M == 2) read_a<0, Q>(buf, ks_f);     // its last MFMA was M == 1
+                    if constexpr (M == 3) read_a<2, Q>(buf, ks_f);
+                    if constexpr (M == 4) read_a<1, Q>(buf, ks_f);     // its last MFMA was M == 3
+                    if constexpr (M == 5) read_a<3, Q>(buf, ks_f);
+                } else {
+                    if constexpr (M == 0) read_b<0, Q>(buf, ks_f);
+                    if constexpr (M == 1) { read_b<1, Q>(buf, ks_f); read_a<0, Q>(buf, ks_f); }
+                    if constexpr (M == 2) read_a<1, Q>(buf, ks_f);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            after(IntC<M>());
+            sub<P, FETCH, M + 1>(acc, buf, ks_f, after);
+        } else {
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    struct Nothing { template <typename I> FX_DEV void operator()(I) const {} };
+
+    // One K-step from `cur` whose successor is in (or on its way to) `nxt`; with MORE the one after that is requested
+    // into `cur`.
+    template <bool MORE>
+    FX_DEV void step(f32x16_t (&acc)[TM][TN], uint8_t* cur, uint8_t* nxt) {
+        fetch_scales();                                  // of the next K-step; they land with its tiles below
+        sub<0, true>(acc, cur, 1, Nothing());
+        // every read of `cur` is out.  Once they and this wave's loads into `nxt` have landed, the barrier makes `nxt`
+        // readable and `cur` writable for everyone; the second half's MFMAs run after it, while the first fragments
+        // of the next K-step are read and the loads of the one after go out.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        // packed here, where nothing is in flight: a use further down would wait for the tile loads issued since
+        int na, nb;
+        pack_scales(na, nb);
+        sub<1, true>(acc, nxt, 0, [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            if constexpr (MORE) static_for<M * PER, (M + 1) * PER>([&](auto i) { issue_one<decltype(i)::value>(cur); });
+        });
+        sca = na;
+        scb = nb;
+    }
+
+    // K loop; leaves the (transposed) accumulators of this wave's sub-tile and ends with a barrier.
+    // first_landed: the loads of K-step 0 have been waited for, with a barrier since.
+    FX_DEV void finish(const Fp8Job<TD>& job, uint8_t* buf0, uint8_t* buf1, f32x16_t (&acc)[TM][TN], bool first_landed) {
+        const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+        const int K = job.K, nfull = K / FP8_BK;
+        // wave-uniform: does any element of this wave's sub-tile exist?
+        const bool live = __builtin_amdgcn_readfirstlane((job.m0 + wm * WM < job.A.ext) && (job.n0 + wn * WN < job.B.ext));
+        auto stage = [&](int kt) { return (kt & 1) ? buf1 : buf0; };
+        if (nfull > 0) {
+            if (nfull > 1) issue(buf1);
+            if (!first_landed) {
+                if (nfull > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LD) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
+            if (!live) {
+                // this wave keeps loading its share of the stages, meets every barrier of the loop below and leaves
+                // the matrix pipe to the wave it shares a SIMD with
+                for (int kt = 0; kt + 1 < nfull; ++kt) {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    __syncthreads();
+                    if (kt + 2 < nfull) issue(stage(kt));
+                }
+            } else {
+                pack_scales(sca, scb);
+                static_for<0, TN>([&](auto j) { read_b<decltype(j)::value, 0>(buf0, 0); });
+                static_for<0, TM>([&](auto i) { read_a<decltype(i)::value, 0>(buf0, 0); });
+                // straight-line K-steps: a branch between the MFMAs lets the compiler sink them all behind the loads
+                for (int kt = 0; kt + 2 < nfull; ++kt) step<true>(acc, stage(kt), stage(kt + 1));
+                if (nfull > 1) step<false>(acc, stage(nfull - 2), stage(nfull - 1));
+                uint8_t* cur = stage(nfull - 1);
+                sub<0, true>(acc, cur, 1, Nothing());
+                sub<1, false>(acc, cur, 0, Nothing());
+            }
+        }
+        if (nfull * FP8_BK < K) {
+            // last partial K-step: through registers, zero behind K.  `buf` was last read two K-steps ago.
+            uint8_t* buf = stage(nfull);
+            const int tid = threadIdx.x;
+            if (nfull > 0) fetch_scales();       // (with no full K-step begin() has requested these)
+            for (int id = tid; id < (BM + BN) * 8; id += NT) {
+                const int r = id >> 3, c = id & 7, k = nfull * FP8_BK + c * 16;
+                const uint8_t* row = r < BM ? job.A.p + a_row(job, r) * job.A.ld
+                                            : job.B.p + (int64_t)min(job.n0 + r - BM, job.B.ext - 1) * job.B.ld;
+                const u32x4_t v = load_chunk(row, k, K);
+                *reinterpret_cast<u32x4_t*>(buf + r * FP8_BK + ((c ^ swz(r)) << 4)) = v;
+            }
+            __syncthreads();
+            if (live) {
+                pack_scales(sca, scb);
+                static_for<0, TN>([&](auto j) { read_b<decltype(j)::value, 0>(buf, 0); });
+                static_for<0, TM>([&](auto i) { read_a<decltype(i)::value, 0>(buf, 0); });
+                sub<0, true>(acc, buf, 1, Nothing());
+                sub<1, false>(acc, buf, 0, Nothing());
+            }
+        }
+        __syncthreads();      // every wave is past its last LDS read: the stages are free
+    }
+};
+
+// ---------------------------------------------------------------- kernels over a list of tiles
+// A Source names the tiles of a launch: total(lane) how many there are, locate(id, lane) where tile `id` lies (a small
+// struct), job(where) its operands.  Counts of experts are read by whole waves (find_group_tile), so every lane calls.
+
+// 256 x 256 tiles, eight waves of 128 x 64, one workgroup per CU that walks the list with the grid as stride: the first
+// K-step of its next tile is requested before the epilogue of the current one.
+// LDS: [stage 0: 64 KB][stage 1: 64 KB, and the epilogue's staging, which reaches 4 KB past it]; the staging may
+// overlap stage 1 because the second K-step of the next tile is issued after the barrier behind the epilogue.
+constexpr int FP8_WALK_BM = 256, FP8_WALK_BN = 256;
+constexpr size_t kFp8WalkLds = 64 * 1024 + epilogue_lds_bytes<8, 64>();
+
+template <int AF, typename TD, bool NT, typename Source>
+__global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    typedef Fp8Loop<AF, TD, FP8_WALK_BM, FP8_WALK_BN, 2, 4> Loop;
+    static_assert(Loop::STAGE == 64 * 1024, "the LDS plan assumes 64 KB stages");
+    uint8_t *buf0 = smem, *buf1 = smem + Loop::STAGE;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int total = src.total(lane);
+    int id = blockIdx.x;
+    if (id >= total) return;
+    Loop loop;
+    auto cur = src.locate(id, total, lane);
+    loop.begin(src.job(cur), buf0);
+    bool landed = false;
+    for (;;) {
+        const int next = id + (int)gridDim.x;
+        const bool more = next < total;
+        auto nxt = cur;
+        if (more) nxt = src.locate(next, total, lane);
+        f32x16_t acc[Loop::TM][Loop::TN];
+        loop.finish(src.job(cur), buf0, buf1, acc, landed);
+        if (more) loop.begin(src.job(nxt), buf0);
+        const Fp8Job<TD> j = src.job(cur);
+        epilogue_tile<bf16, TD, Loop::WM, Loop::WN, true, NT>(acc, j.C, j.D, src.ldc, src.ldd, j.m0 + (wave / 4) * Loop::WM,
+                                                              j.n0 + (wave % 4) * Loop::WN, j.A.ext, j.B.ext, 1.f, j.C != nullptr ? 1.f : 0.f,
+                                                              reinterpret_cast<bf16*>(buf1), wave, lane);
+        if (!more) break;
+        __syncthreads();
+        landed = true;
+        cur = nxt;
+        id = next;
+    }
+}
+
+// 128 x 128 tiles, four waves of 64 x 64, one tile per workgroup; 64 KB of LDS, so two workgroups share a CU and one's
+// epilogue and first loads run under the other's K loop.
+template <int AF, typename TD, typename Source>
+__global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    typedef Fp8Loop<AF, TD, 128, 128, 2, 2> Loop;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int total = src.total(lane);
+    if ((int)blockIdx.x >= total) return;
+    Loop loop;
+    const Fp8Job<TD> j = src.job(src.locate(blockIdx.x, total, lane));
+    loop.begin(j, smem);
+    f32x16_t acc[Loop::TM][Loop::TN];
+    loop.finish(j, smem, smem + Loop::STAGE, acc, false);
+    epilogue_tile<bf16, TD, Loop::WM, Loop::WN>(acc, j.C, j.D, src.ldc, src.ldd, j.m0 + (wave / 2) * Loop::WM,
+                                                j.n0 + (wave % 2) * Loop::WN, j.A.ext, j.B.ext, 1.f, j.C != nullptr ? 1.f : 0.f,
+                                                reinterpret_cast<bf16*>(smem), wave, lane);
+}
+constexpr size_t kFp8Tile128Lds = 64 * 1024;
+static_assert(epilogue_lds_bytes<4, 64>() <= kFp8Tile128Lds, "epilogue staging");
+
+static inline int fp8_cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// One workgroup per CU for the kernels that walk their tiles.
+static inline int fp8_walk_grid() {
+    int dev = 0, n = 0;
+    (void)hipGetDevice(&dev);
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    return n;
+}
+
+// Bytes a scale tensor spans (0: none), and whether lane offsets of 32 bits cover an operand.
+static inline bool fp8_scales_fit(int64_t rows, int64_t s_row, int64_t blocks, int64_t s_k) {
+    if (rows <= 0 || blocks <= 0) return true;
+    if (s_row < 0 || s_k < 0) return false;
+    const double span = (double)(rows - 1) * (double)s_row + (double)(blocks - 1) * (double)s_k;
+    return span < 2147483647.0;
+}
+constexpr int64_t kFp8MaxLd = (int64_t)1 << 23;
+
+// Rows of an operand start at 16-byte addresses.
+static inline bool fp8_bad_rows(const void* p, int64_t ld) { return !aligned16(p) || (ld & 15) != 0; }
+
+}  // namespace fx

@@ -1,0 +1,178 @@
+// Block-scaled 8-bit products grouped by expert (fp8_gemm.hip has the dense one), gfx950.
+//
+//   rows form   D[rows of e] = A[rows of e] B[e]^T           rows of e: COUNTS[e] consecutive expert-sorted rows
+//   wgrad form  D[e] = A_e B_e^T + C[e]                      A_e, B_e: the columns of expert e of transposed operands,
+//                                                            every expert starting at a multiple of 128
+// One launch each; the counts stay on the device.  A workgroup finds its tiles from the counts themselves (a scan
+// over 64 experts per wave step), so there is no plan to make, keep or share.
+#include "fp8_core.h"
+#include "flexhip.h"
+
+namespace fx {
+
+template <typename TD, int SHIFT, int BN>
+struct Fp8GroupedRows {
+    Fp8View A, B;
+    int64_t b_expert, sb_expert;
+    const int32_t* COUNTS;
+    const int32_t* MAP;
+    TD* D;
+    int64_t ldc, ldd, total_rows;
+    int E, src_rows, K, tiles_n;
+    struct Where { int row0, e, rows, m0, n0; };
+    FX_DEV int total(int lane) const { return count_group_tiles<SHIFT>(COUNTS, E, total_rows, lane) * tiles_n; }
+    FX_DEV Where locate(int id, int total, int lane) const {
+        // expert-major, column tile fastest; each XCD (own L2) takes a contiguous band of that order
+        const int p = xcd_band(id, total);
+        const GroupTile t = find_group_tile<SHIFT>(COUNTS, E, p / tiles_n, total_rows, lane);
+        return Where{t.row0, t.e, t.rows, t.m0, (p % tiles_n) * BN};
+    }
+    FX_DEV Fp8Job<TD> job(const Where& w) const {
+        Fp8Job<TD> j{A, B, w.m0, w.n0, K, nullptr, src_rows, nullptr, D + (int64_t)w.row0 * ldd};
+        j.A.ext = w.rows;
+        if (MAP != nullptr) {
+            j.row_map = MAP + w.row0;
+        } else {
+            j.A.p += (int64_t)w.row0 * A.ld;
+            j.A.s += (int64_t)w.row0 * A.s_row;
+        }
+        j.B.p += w.e * b_expert;
+        j.B.s += w.e * sb_expert;
+        return j;
+    }
+};
+
+template <typename TD, int BM, int BN>
+struct Fp8GroupedWgrad {
+    Fp8View A, B;
+    const int32_t* COUNTS;
+    const TD* C;
+    TD* D;
+    int64_t ldc, ldd, c_expert, d_expert, capacity;
+    int E, tiles_m, tiles_n;
+    struct Where { int padded0, e, rows, m0, n0; };
+    FX_DEV int total(int) const { return E * tiles_m * tiles_n; }
+    FX_DEV Where locate(int id, int total, int lane) const {
+        const int p = xcd_band(id, total), per = tiles_m * tiles_n;
+        const int e = p / per, q = p % per;
+        const GroupSpan s = find_group_span(COUNTS, E, e, capacity, lane);
+        return Where{s.padded0, e, s.rows, (q / tiles_n) * BM, (q % tiles_n) * BN};
+    }
+    FX_DEV Fp8Job<TD> job(const Where& w) const {
+        // the places behind an expert's rows hold zeros: whole K-steps
+        Fp8Job<TD> j{A, B, w.m0, w.n0, (w.rows + 127) & ~127, nullptr, 0, C ? C + (int64_t)w.e * c_expert : nullptr, D + (int64_t)w.e * d_expert};
+        j.A.p += w.padded0;
+        j.B.p += w.padded0;
+        j.A.s += (int64_t)(w.padded0 >> 7) * A.s_k;
+        j.B.s += (int64_t)(w.padded0 >> 7) * B.s_k;
+        return j;
+    }
+};
+
+// 256-row tiles when experts average 384 rows or more, else 128-row ones (two workgroups per CU).
+static int fp8_rows_shift(int64_t total_rows, int E) { return total_rows / E >= 384 ? 8 : 7; }
+
+template <int AF, typename TD>
+static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int64_t sb_expert, const int32_t* counts,
+                       const int32_t* map, int64_t a_rows, TD* D, int64_t ldd, int64_t total_rows, int E, int K, hipStream_t stream) {
+    const int N = b.ext;
+    const int shift = fp8_rows_shift(total_rows, E);
+    // at most this many row tiles, whatever the split over the experts
+    const int64_t most = (total_rows >> shift) + (E < total_rows ? E : total_rows);
+    const int tiles_n = fp8_cdiv(N, 1 << shift);
+    if (most * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
+    if (shift == 8) {
+        typedef Fp8GroupedRows<TD, 8, 256> Source;
+        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};
+        const unsigned grid = (unsigned)(most * tiles_n < fp8_walk_grid() ? most * tiles_n : fp8_walk_grid());
+        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+    } else {
+        typedef Fp8GroupedRows<TD, 7, 128> Source;
+        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};
+        auto kern = fp8_tile_kernel128<AF, TD, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8Tile128Lds);
+        kern<<<dim3((unsigned)(most * tiles_n)), 256, kFp8Tile128Lds, stream>>>(src);
+    }
+    FX_CHECK_LAUNCH("fx_fp8_grouped_gemm");
+    return 0;
+}
+
+template <int AF, typename TD>
+static int launch_wgrad(const Fp8View& a, const Fp8View& b, const int32_t* counts, int E, int64_t capacity, const TD* C, int64_t ldc,
+                        int64_t c_expert, TD* D, int64_t ldd, int64_t d_expert, hipStream_t stream) {
+    const int M = a.ext, N = b.ext;
+    const int64_t big = (int64_t)E * fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
+    if (big >= 192) {
+        if (big > 0x7fffffff) FX_FAIL("fx_fp8_grouped_wgrad: too many tiles");
+        typedef Fp8GroupedWgrad<TD, 256, 256> Source;
+        const Source src{a, b, counts, C, D, ldc, ldd, c_expert, d_expert, capacity, E, fp8_cdiv(M, 256), fp8_cdiv(N, 256)};
+        const unsigned grid = (unsigned)(big < fp8_walk_grid() ? big : fp8_walk_grid());
+        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+    } else {
+        const int64_t tiles = (int64_t)E * fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
+        typedef Fp8GroupedWgrad<TD, 128, 128> Source;
+        const Source src{a, b, counts, C, D, ldc, ldd, c_expert, d_expert, capacity, E, fp8_cdiv(M, 128), fp8_cdiv(N, 128)};
+        auto kern = fp8_tile_kernel128<AF, TD, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8Tile128Lds);
+        kern<<<dim3((unsigned)tiles), 256, kFp8Tile128Lds, stream>>>(src);
+    }
+    FX_CHECK_LAUNCH("fx_fp8_grouped_wgrad");
+    return 0;
+}
+
+}  // namespace fx
+
+using namespace fx;
+
+extern "C" int fx_fp8_grouped_gemm(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k,
+                                   const int32_t* row_map, int64_t a_rows, const void* B, int64_t ldb, int64_t b_expert,
+                                   const void* SB, int64_t sb_row, int64_t sb_k, int64_t sb_expert, int b_tiles,
+                                   const int32_t* counts, int E, int64_t total_rows, void* D, int64_t ldd, int N, int K, int d_dt,
+                                   hipStream_t stream) {
+    if (E <= 0 || total_rows < 0 || N < 0 || K < 0) FX_FAIL("fx_fp8_grouped_gemm: bad shape");
+    if (!is_fp8_dt(a_dt)) FX_FAIL("fx_fp8_grouped_gemm: unsupported 8-bit dtype enum %d", a_dt);
+    if (d_dt != DT_F32 && d_dt != DT_F16 && d_dt != DT_BF16) FX_FAIL("fx_fp8_grouped_gemm: unsupported output dtype enum %d", d_dt);
+    if (total_rows > (1 << 24)) FX_FAIL("fx_fp8_grouped_gemm: at most 2^24 expert rows");
+    if (total_rows == 0 || N == 0) return 0;
+    if (!counts || !D || (K > 0 && (!A || !B || !SA || !SB))) FX_FAIL("fx_fp8_grouped_gemm: null pointer");
+    if (K > 0 && (fp8_bad_rows(A, lda) || fp8_bad_rows(B, ldb) || (b_expert & 15))) FX_FAIL("fx_fp8_grouped_gemm: rows of A and B must start at 16-byte addresses");
+    if ((K > 0 && (lda < K || ldb < K)) || ldd < N) FX_FAIL("fx_fp8_grouped_gemm: a row stride is shorter than the row");
+    if (lda >= kFp8MaxLd || ldb >= kFp8MaxLd) FX_FAIL("fx_fp8_grouped_gemm: row strides must be below 2^23 bytes");
+    if (row_map ? (a_rows <= 0 || a_rows > 0x7fffffff) : a_rows < total_rows) FX_FAIL("fx_fp8_grouped_gemm: A has %lld rows", (long long)a_rows);
+    if (row_map && (uint64_t)a_rows * (uint64_t)lda >= (1ull << 32)) FX_FAIL("fx_fp8_grouped_gemm: a gathered A must stay below 4 GB");
+    const int kb = fp8_cdiv(K, FP8_BK);
+    if (!fp8_scales_fit(a_rows, sa_row, kb, sa_k) || !fp8_scales_fit(b_tiles ? fp8_cdiv(N, 128) : N, sb_row, kb, sb_k) || sb_expert < 0 || b_expert < 0)
+        FX_FAIL("fx_fp8_grouped_gemm: the scales of A, and those of an expert's B, must span less than 2 GB, with no negative stride");
+    const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, 0, 0};
+    const Fp8View b{(const uint8_t*)B, (const uint8_t*)SB, (int)ldb, (int)sb_row, (int)sb_k, b_tiles ? 7 : 0, N};
+    int rc = -1;
+    FX_DISPATCH_FP8(a_dt, AF, FX_DISPATCH_DTYPE(d_dt, TD, rc = launch_rows<AF, TD>(a, b, b_expert, sb_expert, counts, row_map, a_rows, (TD*)D, ldd, total_rows, E, K, stream)));
+    return rc;
+}
+
+extern "C" int fx_fp8_grouped_wgrad(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k, const void* B,
+                                    int64_t ldb, const void* SB, int64_t sb_row, int64_t sb_k, const int32_t* counts, int E,
+                                    int64_t capacity, const void* C, int64_t ldc, int64_t c_expert, void* D, int64_t ldd,
+                                    int64_t d_expert, int M, int N, int d_dt, hipStream_t stream) {
+    if (E <= 0 || capacity < 0 || (capacity & 127) || M < 0 || N < 0) FX_FAIL("fx_fp8_grouped_wgrad: bad shape");
+    if (!is_fp8_dt(a_dt)) FX_FAIL("fx_fp8_grouped_wgrad: unsupported 8-bit dtype enum %d", a_dt);
+    if (d_dt != DT_F32 && d_dt != DT_F16 && d_dt != DT_BF16) FX_FAIL("fx_fp8_grouped_wgrad: unsupported output dtype enum %d", d_dt);
+    if (capacity >= kFp8MaxLd) FX_FAIL("fx_fp8_grouped_wgrad: at most 2^23 expert rows");
+    if (M == 0 || N == 0) return 0;
+    if (!counts || !D || (capacity > 0 && (!A || !B || !SA || !SB))) FX_FAIL("fx_fp8_grouped_wgrad: null pointer");
+    if (capacity > 0 && (fp8_bad_rows(A, lda) || fp8_bad_rows(B, ldb))) FX_FAIL("fx_fp8_grouped_wgrad: rows of A and B must start at 16-byte addresses");
+    if (lda < capacity || ldb < capacity || ldd < N || (C && ldc < N)) FX_FAIL("fx_fp8_grouped_wgrad: a row stride is shorter than the row");
+    if (lda >= kFp8MaxLd || ldb >= kFp8MaxLd) FX_FAIL("fx_fp8_grouped_wgrad: row strides must be below 2^23 bytes");
+    if (!fp8_scales_fit(M, sa_row, capacity / 128, sa_k) || !fp8_scales_fit(N, sb_row, capacity / 128, sb_k))
+        FX_FAIL("fx_fp8_grouped_wgrad: a scale tensor must span less than 2 GB, with no negative stride");
+    if ((int64_t)E * fp8_cdiv(M, 128) * fp8_cdiv(N, 128) > 0x7fffffff) FX_FAIL("fx_fp8_grouped_wgrad: too many tiles");
+    const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, 0, M};
+    const Fp8View b{(const uint8_t*)B, (const uint8_t*)SB, (int)ldb, (int)sb_row, (int)sb_k, 0, N};
+    int rc = -1;
+    FX_DISPATCH_FP8(a_dt, AF, FX_DISPATCH_DTYPE(d_dt, TD, rc = launch_wgrad<AF, TD>(a, b, counts, E, capacity, (const TD*)C, ldc, c_expert, (TD*)D, ldd, d_expert, stream)));
+    return rc;
+}

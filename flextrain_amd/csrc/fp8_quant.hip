@@ -92,8 +92,8 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
     int live = (int)min((int64_t)128, rows - first);
     if (GROUPED) {
         // every expert's rows start at a multiple of 128 of the row axis written here
-        const GroupTile t = find_group_tile<7>(COUNTS, E, tr, rows, lane);
-        first = t.row0 + t.m0;
+        const GroupTile t = find_group_tile<7>(COUNTS, E, (int)tr, rows, lane);
+        first = (int64_t)t.row0 + t.m0;
         live = max(0, min(128, t.rows - t.m0));
     }
     const int64_t col = tc * 128 + c * 8;

@@ -19,8 +19,8 @@ OUT = os.path.join(HERE, "_build")
 LIB = os.path.join(OUT, "libflexhip_hostsim.so")
 CLANG = "/opt/rocm/lib/llvm/bin/clang++"
 SOURCES = ("rmsnorm.hip", "rope.hip", "glu.hip", "softmax_ce.hip", "adamw.hip", "moe_route.hip", "moe_data.hip", "embed.hip",
-           "gemm.hip", "gemm_glu.hip", "gemm_ksum.hip", "gemm_segments.hip", "grouped_gemm.hip", "stream.hip", "fp8_quant.hip", "add_rmsnorm.hip", "fp8_gemm.hip")
-HEADERS = ("common.h", "gemm_core.h", "gemm_core2.h", "fp8.h")
+           "gemm.hip", "gemm_glu.hip", "gemm_ksum.hip", "gemm_segments.hip", "grouped_gemm.hip", "stream.hip", "fp8_quant.hip", "add_rmsnorm.hip", "fp8_gemm.hip", "fp8_grouped.hip")
+HEADERS = ("common.h", "gemm_core.h", "gemm_core2.h", "fp8.h", "fp8_core.h")
 
 
 def _marker():
@@ -160,7 +160,7 @@ def build(force=False):
     objects = []
     for name in HEADERS:                 # the headers with inline assembly are rewritten too and found first
         with open(os.path.join(OUT, name), "w") as f:
-            f.write(rewrite_lockstep(rewrite_asm(open(os.path.join(CSRC, name)).read())))
+            f.write(rewrite_lockstep(rewrite_asm(rewrite_dynamic_lds(open(os.path.join(CSRC, name)).read()))))
     for name in SOURCES:
         text = open(os.path.join(CSRC, name)).read()
         cpp = os.path.join(OUT, name.replace(".hip", "_hostsim.cpp"))

@@ -236,6 +236,14 @@ inline float fp8_value(unsigned char b, bool e5m2) {
     else v = ex ? ldexpf((float)(mant + (1 << mbits)), ex - bias - mbits) : ldexpf((float)mant, 1 - bias - mbits);
     return b & 0x80 ? -v : v;
 }
+struct Fp8Table {
+    float value[2][256];
+    Fp8Table() {
+        for (int e = 0; e < 2; ++e)
+            for (int b = 0; b < 256; ++b) value[e][b] = fp8_value((unsigned char)b, e == 1);
+    }
+};
+inline const Fp8Table& fp8_table() { static const Fp8Table t; return t; }
 // nearest even; finite values past the largest number become NaN (e4m3) or infinity (e5m2)
 inline unsigned char fp8_code(float x, bool e5m2) {
     const int mbits = e5m2 ? 2 : 3, low = e5m2 ? -14 : -6;
@@ -270,19 +278,32 @@ inline Acc mfma_scale(Frag a, Frag b, Acc c, int fmt_a, int fmt_b, int opsel_a, 
     const unsigned char *pa = reinterpret_cast<const unsigned char*>(&a), *pb = reinterpret_cast<const unsigned char*>(&b);
     const int ba = (scale_a >> (8 * opsel_a)) & 255, bb = (scale_b >> (8 * opsel_b)) & 255;
     const float sa = ba == 255 ? NAN : ldexpf(1.f, ba - 127), sb = bb == 255 ? NAN : ldexpf(1.f, bb - 127);
-    for (int j = 0; j < 32; ++j) { mine[j] = fp8_value(pa[j], fmt_a == 1) * sa; mine[32 + j] = fp8_value(pb[j], fmt_b == 1) * sb; }
+    const float *ta = fp8_table().value[fmt_a == 1], *tb = fp8_table().value[fmt_b == 1];
+    for (int j = 0; j < 32; ++j) { mine[j] = ta[pa[j]] * sa; mine[32 + j] = tb[pb[j]] * sb; }
     sync_wave();
     for (int v = 0; v < N * N / 64; ++v) {
         const unsigned row = N == 32 ? 8u * (v / 4) + 4u * (l / 32) + (unsigned)(v % 4) : 4u * (l / 16) + (unsigned)v;
         float sum = c[v];
         for (int q = 0; q < K_LANES; ++q) {
             const float *x = g_wave_f8[w][row + N * q], *y = g_wave_f8[w][l % N + N * q] + 32;
-            for (int k = 0; k < 32; ++k) sum += x[k] * y[k];
+            float part[8] = {0, 0, 0, 0, 0, 0, 0, 0};          // eight partial sums: the compiler's vectors
+            for (int k = 0; k < 32; k += 8)
+                for (int u = 0; u < 8; ++u) part[u] += x[k + u] * y[k + u];
+            for (int u = 0; u < 8; ++u) sum += part[u];
         }
         c[v] = sum;
     }
     sync_wave();
     return c;
+}
+
+// v_permlane32_swap: the upper 32 lanes of the first operand change places with the lower 32 of the second.
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+inline u32x2_t permlane32_swap(unsigned a, unsigned b) {
+    const unsigned l = flat_thread() & 63u;
+    const unsigned b_lo = exchange(b, (int)(l & 31u)), a_hi = exchange(a, (int)((l & 31u) + 32u));
+    u32x2_t out = {l < 32 ? a : b_lo, l < 32 ? a_hi : b};
+    return out;
 }
 
 // ds_read_b64_tr_b16: inside each group of 16 lanes, lane s receives, for j = 0 .. 3, element s % 4 of the
@@ -314,6 +335,7 @@ inline unsigned perm_b32(unsigned hi, unsigned lo, unsigned sel) {
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) hostsim::mfma32x32x16(a, b, c)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<32>(a, b, c, fa, fb, oa, sa, ob, sb)
 #define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<16>(a, b, c, fa, fb, oa, sa, ob, sb)
+#define __builtin_amdgcn_permlane32_swap(a, b, fi, bc) hostsim::permlane32_swap(a, b)
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, false)
 #define __builtin_amdgcn_cvt_pk_bf8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, true)
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) hostsim::ds_read_tr16<short __attribute__((ext_vector_type(4)))>((const void*)(p))

@@ -232,6 +232,18 @@ def test_matmul(dev, m, n, k, fmt, b_tiles):
     assert torch.equal(acc, out)
 
 
+@pytest.mark.parametrize("m,n,k", [(8200, 1540, 200), (2050, 6300, 384), (300, 12000, 128)])
+def test_matmul_many_tiles(dev, m, n, k):
+    """Enough tiles to fill the GPU: the launch whose workgroups walk several 256 x 256 tiles."""
+    g = gen(m)
+    a, sa, av = operand(dev, values(g, m, k, sigma=1e-3), E5M2)
+    b, sb, bv = operand(dev, values(g, n, k, sigma=k ** -0.5), tiles=True)
+    ref = av @ bv.t()
+    c = values(g, m, n, sigma=float(ref.std()))
+    check(ops.flextrain_fp8_matmul(a, sa, b, sb), ref, av, bv)
+    check(ops.flextrain_fp8_matmul(a, sa, b, sb, C=c.to(dev)), ref + c.double(), av, bv, c)
+
+
 def test_matmul_tiles_on_both_sides_and_strides(dev):
     g = gen(3)
     x, w = values(g, 200, 384), values(g, 300, 384)
@@ -327,7 +339,7 @@ def test_grouped_matmul_leaves_rows_behind_the_last_expert(dev):
 
 @pytest.mark.parametrize("fmt", [E4M3, E5M2])
 @pytest.mark.parametrize("counts,m,n", [(c, m, n) for c, m, n in [([5], 64, 128), ([0, 0, 3, 0], 40, 256), ([128, 1, 0, 127, 129, 0], 130, 200),
-                                                                  ([1] * 70, 24, 40), ([0] * 66 + [300, 7], 257, 136), ([600, 0, 50], 136, 264)]],
+                                                                  ([1] * 70, 24, 40), ([1, 0, 2] * 66, 24, 40), ([0] * 66 + [300, 7], 257, 136), ([600, 0, 50], 136, 264)]],
                          ids=lambda v: f"{len(v)}x{sum(v)}" if isinstance(v, list) else str(v))
 def test_grouped_wgrad(dev, counts, m, n, fmt):
     g = gen(m + n)
