@@ -368,6 +368,131 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
 constexpr size_t kFp8Tile128Lds = 64 * 1024;
 static_assert(epilogue_lds_bytes<4, 64>() <= kFp8Tile128Lds, "epilogue staging");
 
+// Small products: one workgroup per tile of 16 MT x 16 NT, its NW waves share the contraction (wave w takes K-steps
+// w, w + NW, ..) and add up through LDS in ascending order.  Operands go straight from memory into registers: with
+// few rows nothing is used twice by a workgroup, so LDS staging and its barriers would only add latency, and with one
+// launch and one pass a single token costs the weight's bytes.  The matrix instruction is the 16 x 16 x 128 one.
+// A lane takes bytes [16 h, 16 h + 16) and [64 + 16 h, ..) of its row's 128 (h = lane / 16), so one load instruction
+// of a wave covers 64 contiguous bytes of each of 16 rows; A and B use the same order of k, which is all that matters.
+typedef float f32x4v_t __attribute__((ext_vector_type(4)));
+
+template <int AF>
+FX_DEV f32x4v_t mfma_fp8_16(const i32x8_t& b, const i32x8_t& a, f32x4v_t c, int sb, int sa) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, AF == DT_E4M3 ? 0 : 1, 0, sb, 0, sa);
+}
+
+template <int AF, typename TD, int MT, int NT, int NW, int U, typename Source>
+__global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
+    __shared__ f32x4v_t red[NW][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int total = src.total(lane);
+    if ((int)blockIdx.x >= total) return;
+    const Fp8Job<TD> j = src.job(src.locate(blockIdx.x, total, lane));
+    const int r = lane & 15, h = lane >> 4;
+    const uint8_t *pa[MT], *pb[NT], *sa[MT], *sb[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int g = min(j.m0 + i * 16 + r, j.A.ext - 1);
+        const int row = j.row_map != nullptr ? min(max(j.row_map[g], 0), j.src_rows - 1) : g;
+        pa[i] = j.A.p + (int64_t)row * j.A.ld + h * 16;
+        sa[i] = j.A.s + (int64_t)(row >> j.A.s_shift) * j.A.s_row;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int row = min(j.n0 + i * 16 + r, j.B.ext - 1);
+        pb[i] = j.B.p + (int64_t)row * j.B.ld + h * 16;
+        sb[i] = j.B.s + (int64_t)(row >> j.B.s_shift) * j.B.s_row;
+    }
+    f32x4v_t acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[i][n] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
+    union Frag { i32x8_t f; u32x4_t q[2]; };
+    const int K = j.K, nfull = K / FP8_BK;
+    auto load = [&](Frag (&fa)[MT], Frag (&fb)[NT], int (&ca)[MT], int (&cb)[NT], int kb) {
+        const int64_t k = (int64_t)kb * FP8_BK;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            fb[n].q[0] = ldg16(pb[n] + k);
+            fb[n].q[1] = ldg16(pb[n] + k + 64);
+            cb[n] = sb[n][(int64_t)kb * j.B.s_k];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            fa[i].q[0] = ldg16(pa[i] + k);
+            fa[i].q[1] = ldg16(pa[i] + k + 64);
+            ca[i] = sa[i][(int64_t)kb * j.A.s_k];
+        }
+    };
+    auto multiply = [&](const Frag (&fa)[MT], const Frag (&fb)[NT], const int (&ca)[MT], const int (&cb)[NT]) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[i][n] = mfma_fp8_16<AF>(fb[n].f, fa[i].f, acc[i][n], cb[n], ca[i]);
+    };
+    Frag fa[U][MT], fb[U][NT];
+    int ca[U][MT], cb[U][NT];
+    int kb = wave;
+    for (; kb + (U - 1) * NW < nfull; kb += U * NW) {       // U K-steps in flight
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(fa[u], fb[u], ca[u], cb[u], kb + u * NW);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(fa[u], fb[u], ca[u], cb[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (kb + u * NW < nfull) load(fa[u], fb[u], ca[u], cb[u], kb + u * NW);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (kb + u * NW < nfull) multiply(fa[u], fb[u], ca[u], cb[u]);
+    if (nfull * FP8_BK < K && nfull % NW == wave) {         // last partial K-step: zero behind K
+        const int k = nfull * FP8_BK;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            fb[0][n].q[0] = load_chunk(pb[n] - h * 16, k + h * 16, K);
+            fb[0][n].q[1] = load_chunk(pb[n] - h * 16, k + 64 + h * 16, K);
+            cb[0][n] = sb[n][(int64_t)nfull * j.B.s_k];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            fa[0][i].q[0] = load_chunk(pa[i] - h * 16, k + h * 16, K);
+            fa[0][i].q[1] = load_chunk(pa[i] - h * 16, k + 64 + h * 16, K);
+            ca[0][i] = sa[i][(int64_t)nfull * j.A.s_k];
+        }
+        multiply(fa[0], fb[0], ca[0], cb[0]);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) red[wave][i * NT + n][lane] = acc[i][n];
+    __syncthreads();
+    // lane holds D[m = lane % 16][n = 4 (lane / 16) .. + 3] of a 16 x 16 block; wave t % NW finishes block t
+    const bool vec = (src.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(j.D) % (4 * sizeof(TD))) == 0 &&
+                     (j.C == nullptr || ((src.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(j.C) % (4 * sizeof(TD))) == 0));
+    for (int t = wave; t < MT * NT; t += NW) {
+        f32x4v_t s = red[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) s += red[w][t][lane];
+        const int m = j.m0 + (t / NT) * 16 + r, n = j.n0 + (t % NT) * 16 + h * 4;
+        if (m >= j.A.ext) continue;
+        typedef TD t4_t __attribute__((ext_vector_type(4)));
+        TD* d = j.D + (int64_t)m * src.ldd + n;
+        const TD* c = j.C != nullptr ? j.C + (int64_t)m * src.ldc + n : nullptr;
+        if (vec && n + 4 <= j.B.ext) {
+            if (c != nullptr) {
+                const t4_t cv = *reinterpret_cast<const t4_t*>(c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += (float)cv[e];
+            }
+            const t4_t o = {(TD)s[0], (TD)s[1], (TD)s[2], (TD)s[3]};
+            *reinterpret_cast<t4_t*>(d) = o;
+        } else {
+            for (int e = 0; e < 4 && n + e < j.B.ext; ++e) d[e] = (TD)(c != nullptr ? s[e] + (float)c[e] : s[e]);
+        }
+    }
+}
+
 static inline int fp8_cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // One workgroup per CU for the kernels that walk their tiles.

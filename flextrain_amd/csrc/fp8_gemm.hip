@@ -70,11 +70,14 @@ __global__ __launch_bounds__(256) void fp8_split_reduce_kernel(const float* __re
     }
 }
 
-struct Fp8Plan { int tile, splits, k_slice; };      // tile 256 or 128
+struct Fp8Plan { int tile, splits, k_slice; };      // tile 256 or 128; 16, 32, 64: the small kernel with that many rows
 
 // 256 x 256 tiles (one workgroup per CU) when there are enough of them to fill the GPU; else 128 x 128, with the
 // contraction cut into slices of at least 4 K-steps while the workgroups still do not fill it.
 static Fp8Plan fp8_plan(int M, int N, int K) {
+    if (M <= 16) return Fp8Plan{16, 1, K};
+    if (M <= 32) return Fp8Plan{32, 1, K};
+    if (M <= 64) return Fp8Plan{64, 1, K};
     const int64_t big = (int64_t)fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
     if (big >= 192) return Fp8Plan{256, 1, K};
     const int64_t small = (int64_t)fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
@@ -104,6 +107,18 @@ static int launch_dense(const Fp8View& a, const Fp8View& b, const TD* C, int64_t
         FX_CHECK_LAUNCH("fx_fp8_gemm");
         return 0;
     }
+#define FX_SMALL(MT, NT, NW, U)                                                                              \
+    if (p.tile == 16 * MT) {                                                                                  \
+        typedef Fp8Dense<TD, 16 * MT, 16 * NT> Source;                                                        \
+        const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(M, 16 * MT), fp8_cdiv(N, 16 * NT)};                \
+        fp8_small_kernel<AF, TD, MT, NT, NW, U, Source><<<dim3((unsigned)(src.tiles_m * src.tiles_n)), NW * 64, 0, stream>>>(src); \
+        FX_CHECK_LAUNCH("fx_fp8_gemm");                                                                       \
+        return 0;                                                                                             \
+    }
+    FX_SMALL(1, 1, 8, 4)
+    FX_SMALL(2, 2, 8, 2)
+    FX_SMALL(4, 2, 4, 2)
+#undef FX_SMALL
     const int tiles_m = fp8_cdiv(M, 128), tiles_n = fp8_cdiv(N, 128);
     if (p.splits <= 1) {
         const Fp8Dense<TD, 128, 128> src{a, b, C, D, ldc, ldd, K, tiles_m, tiles_n};

@@ -69,8 +69,12 @@ struct Fp8GroupedWgrad {
     }
 };
 
-// 256-row tiles when experts average 384 rows or more, else 128-row ones (two workgroups per CU).
-static int fp8_rows_shift(int64_t total_rows, int E) { return total_rows / E >= 384 ? 8 : 7; }
+// Tile rows (their logarithm): 256 when experts average 384 rows or more, 128 (two workgroups per CU), and the small
+// kernel's 64, 32 or 16 when they average fewer than that.
+static int fp8_rows_shift(int64_t total_rows, int E) {
+    const int64_t avg = total_rows / E;
+    return avg >= 384 ? 8 : avg >= 64 ? 7 : avg >= 32 ? 6 : avg >= 16 ? 5 : 4;
+}
 
 template <int AF, typename TD>
 static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int64_t sb_expert, const int32_t* counts,
@@ -79,7 +83,7 @@ static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int
     const int shift = fp8_rows_shift(total_rows, E);
     // at most this many row tiles, whatever the split over the experts
     const int64_t most = (total_rows >> shift) + (E < total_rows ? E : total_rows);
-    const int tiles_n = fp8_cdiv(N, 1 << shift);
+    const int tiles_n = fp8_cdiv(N, shift >= 7 ? 1 << shift : shift == 4 ? 16 : 32);
     if (most * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
     if (shift == 8) {
         typedef Fp8GroupedRows<TD, 8, 256> Source;
@@ -88,6 +92,15 @@ static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int
         auto kern = fp8_walk_kernel<AF, TD, false, Source>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
         kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+#define FX_SMALL(SHIFT, MT, NT, NW, U)                                                                       \
+    } else if (shift == SHIFT) {                                                                              \
+        typedef Fp8GroupedRows<TD, SHIFT, 16 * NT> Source;                                                    \
+        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n}; \
+        fp8_small_kernel<AF, TD, MT, NT, NW, U, Source><<<dim3((unsigned)(most * tiles_n)), NW * 64, 0, stream>>>(src);
+    FX_SMALL(4, 1, 1, 8, 4)
+    FX_SMALL(5, 2, 2, 8, 2)
+    FX_SMALL(6, 4, 2, 4, 2)
+#undef FX_SMALL
     } else {
         typedef Fp8GroupedRows<TD, 7, 128> Source;
         const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};

@@ -20,9 +20,11 @@ rows start at 16-byte addresses.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
-from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, require_same_device, stream_ptr
+from .._lib import check, dtype_enum, fp8_enum, lib, on_device, raw_stream, require_same_device
 
 _E8M0 = torch.float8_e8m0fnu
 
@@ -35,50 +37,63 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-def _fp8_rows(lead, rows, cols, dtype, device):
-    """Uninitialised 8-bit values ``(*lead, rows, cols)`` whose rows start at multiples of 16 bytes."""
-    return torch.empty(*lead, rows, _round_up(cols, 16), dtype=dtype, device=device)[..., :cols]
+def _fp8_rows(batch, rows, cols, dtype, device):
+    """Uninitialised 8-bit values ``(rows, cols)``, or ``(batch, rows, cols)`` when ``batch`` is not None, whose rows
+    start at multiples of 16 bytes."""
+    ld = _round_up(cols, 16)
+    if batch is None:
+        q = torch.empty((rows, ld), dtype=dtype, device=device)
+        return q if ld == cols else q[:, :cols]
+    return torch.empty((batch, rows, ld), dtype=dtype, device=device)[..., :cols]
 
 
-def _scale_store(lead, rows, blocks, device):
-    """Uninitialised scales ``(*lead, rows, blocks)``, the block index outermost in memory."""
-    return torch.empty(*lead, blocks, rows, dtype=_E8M0, device=device).transpose(-1, -2)
+def _scale_store(batch, rows, blocks, device):
+    """Uninitialised scales ``(rows, blocks)`` / ``(batch, rows, blocks)``, the block index outermost in memory."""
+    if batch is None:
+        return torch.empty((blocks, rows), dtype=_E8M0, device=device).t()
+    return torch.empty((batch, blocks, rows), dtype=_E8M0, device=device).transpose(1, 2)
 
 
 def _input_matrix(X, op):
-    if X.dim() not in (2, 3):
-        raise ValueError(f"{op}: X must be (rows, cols) or (batch, rows, cols), got {X.dim()} dims")
-    if X.shape[-1] == 0:
+    """(batch or None, rows, cols, row stride, batch stride) of a matrix to quantise."""
+    shape, stride = X.shape, X.stride()
+    if len(shape) not in (2, 3):
+        raise ValueError(f"{op}: X must be (rows, cols) or (batch, rows, cols), got {len(shape)} dims")
+    rows, cols = shape[-2:]
+    if cols == 0:
         raise ValueError(f"{op}: X has no columns")
-    if X.shape[-1] > 1 and X.stride(-1) != 1:
+    if cols > 1 and stride[-1] != 1:
         raise ValueError(f"{op}: X must have unit column stride")
     # a dimension of one has no stride of its own
-    ldx = X.stride(-2) if X.shape[-2] > 1 else X.shape[-1]
-    if ldx < X.shape[-1] or (X.dim() == 3 and X.shape[0] > 1 and X.stride(0) < 0):
+    ldx = stride[-2] if rows > 1 else cols
+    if ldx < cols:
         raise ValueError(f"{op}: the rows of X overlap")
-    return ldx, X.stride(0) if X.dim() == 3 else 0
+    if len(shape) == 2:
+        return None, rows, cols, ldx, 0
+    return shape[0], rows, cols, ldx, stride[0]
 
 
 def _quantize(X, dtype, tiles, both, op):
-    ldx, x_batch = _input_matrix(X, op)
+    batch, rows, cols, ldx, x_batch = _input_matrix(X, op)
     require_same_device(X, op=op)
-    lead, (rows, cols) = X.shape[:-2], X.shape[-2:]
-    batch = X.shape[0] if X.dim() == 3 else 1
-    q = _fp8_rows(lead, rows, cols, dtype, X.device)
-    s = _scale_store(lead, _blocks(rows) if tiles else rows, _blocks(cols), X.device)
+    x_dt, q_dt, device = dtype_enum(X.dtype), fp8_enum(dtype), X.device
+    rb, cb = _blocks(rows), _blocks(cols)
+    s_rows = rb if tiles else rows
+    q, s = _fp8_rows(batch, rows, cols, dtype, device), _scale_store(batch, s_rows, cb, device)
     qt = st = None
+    t_rows = 0
     if both:
-        qt = _fp8_rows(lead, cols, rows, dtype, X.device)
-        st = _scale_store(lead, _blocks(cols) if tiles else cols, _blocks(rows), X.device)
+        t_rows = cb if tiles else cols
+        qt, st = _fp8_rows(batch, cols, rows, dtype, device), _scale_store(batch, t_rows, rb, device)
     if rows == 0 or batch == 0:
         return q, s, qt, st
     ldq, ldt = _round_up(cols, 16), _round_up(rows, 16)
     with on_device(X):
         rc = lib().fx_fp8_quantize(
-            ptr(X), ldx, x_batch, batch, rows, cols, dtype_enum(X.dtype), fp8_enum(dtype), 1 if tiles else 0,
-            ptr(q), ldq, rows * ldq, ptr(s), s.shape[-2], s.shape[-2] * s.shape[-1],
-            ptr(qt), ldt, cols * ldt, ptr(st), st.shape[-2] if both else 0, st.shape[-2] * st.shape[-1] if both else 0,
-            stream_ptr(X.device))
+            X.data_ptr(), ldx, x_batch, 1 if batch is None else batch, rows, cols, x_dt, q_dt, 1 if tiles else 0,
+            q.data_ptr(), ldq, rows * ldq, s.data_ptr(), s_rows, s_rows * cb,
+            qt.data_ptr() if both else None, ldt, cols * ldt, st.data_ptr() if both else None, t_rows, t_rows * rb,
+            raw_stream(X))
     check(rc, "fx_fp8_quantize")
     return q, s, qt, st
 
@@ -123,48 +138,48 @@ def flextrain_fp8_quantize_grouped_cols(X, counts, dtype=torch.float8_e4m3fn, ro
     op = "flextrain_fp8_quantize_grouped_cols"
     if X.dim() != 2:
         raise ValueError(f"{op}: X must be (rows, cols)")
-    ldx, _ = _input_matrix(X, op)
+    _, x_rows, cols, ldx, _ = _input_matrix(X, op)
     E = _counts_of(counts, op)
-    rows = X.shape[0] if row_sources is None else _sources_of(row_sources, op)
+    rows = x_rows if row_sources is None else _sources_of(row_sources, op)
     require_same_device(X, counts, row_sources, op=op)
-    if rows > 0 and X.shape[0] == 0:
+    if rows > 0 and x_rows == 0:
         raise ValueError(f"{op}: X has no rows")
     if rows > 1 << 24:
         raise ValueError(f"{op}: at most 2**24 expert rows")
-    cols = X.shape[1]
-    cap = int(lib().fx_fp8_grouped_capacity(rows, E))
-    qt = torch.empty(cols, cap, dtype=dtype, device=X.device)
-    st = _scale_store((), cols, cap // 128, X.device)
-    q_dt = fp8_enum(dtype)
+    x_dt, q_dt = dtype_enum(X.dtype), fp8_enum(dtype)
+    cap = (rows + 127 * E) // 128 * 128          # fx_fp8_grouped_capacity
+    qt = torch.empty((cols, cap), dtype=dtype, device=X.device)
+    st = _scale_store(None, cols, cap // 128, X.device)
     if cap > 0:
         with on_device(X):
-            rc = lib().fx_fp8_quantize_grouped_cols(ptr(X), ldx, X.shape[0], rows, cols, dtype_enum(X.dtype), q_dt,
-                                                    ptr(counts), E, ptr(row_sources), ptr(qt), cap, ptr(st), cols,
-                                                    stream_ptr(X.device))
+            rc = lib().fx_fp8_quantize_grouped_cols(X.data_ptr(), ldx, x_rows, rows, cols, x_dt, q_dt, counts.data_ptr(), E,
+                                                    None if row_sources is None else row_sources.data_ptr(),
+                                                    qt.data_ptr(), cap, st.data_ptr(), cols, raw_stream(X))
         check(rc, "fx_fp8_quantize_grouped_cols")
     return qt, st
 
 
-def _values(t, name, op):
-    """Row stride of an 8-bit operand ``(..., rows, cols)``."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+def _values(t, rows, cols, stride, name, op):
+    """Row stride of an 8-bit operand ``(.., rows, cols)``."""
+    if cols > 1 and stride[-1] != 1:
         raise ValueError(f"{op}: {name} must have unit stride along the contraction")
-    ld = t.stride(-2) if t.shape[-2] > 1 else _round_up(t.shape[-1], 16)
-    if t.numel() and (ld % 16 or ld < t.shape[-1] or t.data_ptr() % 16):
+    ld = stride[-2] if rows > 1 else _round_up(cols, 16)
+    if rows and cols and (ld % 16 or ld < cols or t.data_ptr() % 16):
         raise ValueError(f"{op}: the rows of {name} must start at 16-byte addresses (they are {ld} bytes apart)")
     return ld
 
 
 def _scales(s, rows, blocks, tiles_allowed, name, op):
-    """(row stride, block stride, 1 for 128-row tiles) of an operand's scales ``(..., rows | row blocks, blocks)``."""
+    """(row stride, block stride, 1 for 128-row tiles) of an operand's scales ``(.., rows | row blocks, blocks)``."""
     if s.dtype != _E8M0:
         raise TypeError(f"{op}: {name} must be {_E8M0}, got {s.dtype}")
-    got = tuple(s.shape[-2:])
-    if got == (rows, blocks):
-        return s.stride(-2), s.stride(-1), 0
-    if tiles_allowed and got == (_blocks(rows), blocks):
-        return s.stride(-2), s.stride(-1), 1
-    raise ValueError(f"{op}: {name} has shape {tuple(s.shape)}, expected {(rows, blocks)}"
+    got, stride = s.shape, s.stride()
+    if got[-1] == blocks:
+        if got[-2] == rows:
+            return stride[-2], stride[-1], 0
+        if tiles_allowed and got[-2] == _blocks(rows):
+            return stride[-2], stride[-1], 1
+    raise ValueError(f"{op}: {name} has shape {tuple(got)}, expected {(rows, blocks)}"
                      + (f" or {(_blocks(rows), blocks)}" if tiles_allowed else ""))
 
 
@@ -175,28 +190,39 @@ def _operand_dtypes(A, B, op):
     return a_dt
 
 
+def _addend(t, shape, dtype, name, op):
+    """Row stride (and batch stride) of C or out: the output's shape and dtype, unit column stride."""
+    got, stride = t.shape, t.stride()
+    if got != shape:
+        raise ValueError(f"{op}: {name} has shape {tuple(got)}, expected {tuple(shape)}")
+    if got[-1] > 1 and stride[-1] != 1:
+        raise ValueError(f"{op}: {name} must have unit column stride")
+    if got[-2] > 1 and stride[-2] < got[-1]:
+        raise ValueError(f"{op}: the rows of {name} overlap")
+    if t.dtype != dtype:
+        raise TypeError(f"{op}: {name} is {t.dtype}, the output {dtype}")
+    return stride[-2] if got[-2] > 1 else got[-1], stride[0]
+
+
 def _output(out, shape, out_dtype, C, device, op):
-    """The output tensor; C and out have its shape, its dtype and unit column stride."""
-    for t, name in ((C, "C"), (out, "out")):
-        if t is None:
-            continue
-        if tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{op}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{op}: {name} must have unit column stride")
-        if t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
-            raise ValueError(f"{op}: the rows of {name} overlap")
+    """(output, its dtype's enum, its row and batch strides, those of C): C and out have the output's shape and dtype."""
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else C.dtype if C is not None else torch.bfloat16
-    dtype_enum(out_dtype)
-    for t, name in ((C, "C"), (out, "out")):
-        if t is not None and t.dtype != out_dtype:
-            raise TypeError(f"{op}: {name} is {t.dtype}, the output {out_dtype}")
-    return out if out is not None else torch.empty(shape, dtype=out_dtype, device=device)
+    d_dt = dtype_enum(out_dtype)
+    shape = torch.Size(shape)
+    ldc = c_batch = 0
+    if C is not None:
+        ldc, c_batch = _addend(C, shape, out_dtype, "C", op)
+    if out is not None:
+        ldd, d_batch = _addend(out, shape, out_dtype, "out", op)
+        return out, d_dt, ldd, d_batch, ldc, c_batch
+    D = torch.empty(shape, dtype=out_dtype, device=device)
+    return D, d_dt, shape[-1], shape[-1] * shape[-2], ldc, c_batch
 
 
-def _ld(t):
-    return 0 if t is None else t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+@lru_cache(maxsize=4096)
+def _gemm_ws_bytes(M, N, K):
+    return int(lib().fx_fp8_gemm_ws_bytes(M, N, K))
 
 
 def flextrain_fp8_matmul(A, A_scales, B, B_scales, C=None, out=None, out_dtype=None):
@@ -206,23 +232,25 @@ def flextrain_fp8_matmul(A, A_scales, B, B_scales, C=None, out=None, out_dtype=N
     shape).  ``C`` has the output's shape and dtype and may be ``out`` (a gradient accumulated in place).  Output
     dtype: ``out_dtype``, else that of ``out`` or ``C``, else bf16."""
     op = "flextrain_fp8_matmul"
-    if A.dim() != 2 or B.dim() != 2 or A.shape[1] != B.shape[1]:
-        raise ValueError(f"{op}: A {tuple(A.shape)} and B {tuple(B.shape)} must be (M, K) and (N, K)")
+    a_shape, b_shape = A.shape, B.shape
+    if len(a_shape) != 2 or len(b_shape) != 2 or a_shape[1] != b_shape[1]:
+        raise ValueError(f"{op}: A {tuple(a_shape)} and B {tuple(b_shape)} must be (M, K) and (N, K)")
     a_dt = _operand_dtypes(A, B, op)
-    (M, K), N = A.shape, B.shape[0]
-    lda, ldb = _values(A, "A", op), _values(B, "B", op)
-    sa = _scales(A_scales, M, _blocks(K), True, "A_scales", op)
-    sb = _scales(B_scales, N, _blocks(K), True, "B_scales", op)
+    (M, K), N = a_shape, b_shape[0]
+    kb = _blocks(K)
+    lda, ldb = _values(A, M, K, A.stride(), "A", op), _values(B, N, K, B.stride(), "B", op)
+    sa_row, sa_k, a_tiles = _scales(A_scales, M, kb, True, "A_scales", op)
+    sb_row, sb_k, b_tiles = _scales(B_scales, N, kb, True, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, C, out, op=op)
-    D = _output(out, (M, N), out_dtype, C, A.device, op)
+    D, d_dt, ldd, _, ldc, _ = _output(out, (M, N), out_dtype, C, A.device, op)
     if M == 0 or N == 0:
         return D
-    L = lib()
     with on_device(A):
-        nbytes = int(L.fx_fp8_gemm_ws_bytes(M, N, K))
+        nbytes = _gemm_ws_bytes(M, N, K)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device) if nbytes else None
-        rc = L.fx_fp8_gemm(ptr(A), lda, a_dt, ptr(A_scales), *sa, ptr(B), ldb, ptr(B_scales), *sb, ptr(C), _ld(C), ptr(D),
-                           _ld(D), M, N, K, dtype_enum(D.dtype), ptr(ws), nbytes, stream_ptr(A.device))
+        rc = lib().fx_fp8_gemm(A.data_ptr(), lda, a_dt, A_scales.data_ptr(), sa_row, sa_k, a_tiles, B.data_ptr(), ldb,
+                               B_scales.data_ptr(), sb_row, sb_k, b_tiles, None if C is None else C.data_ptr(), ldc,
+                               D.data_ptr(), ldd, M, N, K, d_dt, None if ws is None else ws.data_ptr(), nbytes, raw_stream(A))
     check(rc, "fx_fp8_gemm")
     return D
 
@@ -235,32 +263,36 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
     ``row_sources`` (int32, one entry per expert-sorted row) ``A`` is the unsorted matrix and its rows are gathered by
     the tile loads.  Rows of ``out`` behind the last expert's are left as they were."""
     op = "flextrain_fp8_grouped_matmul"
-    if A.dim() != 2 or B.dim() != 3 or A.shape[1] != B.shape[2]:
-        raise ValueError(f"{op}: A {tuple(A.shape)} and B {tuple(B.shape)} must be (rows, K) and (E, N, K)")
+    a_shape, b_shape = A.shape, B.shape
+    if len(a_shape) != 2 or len(b_shape) != 3 or a_shape[1] != b_shape[2]:
+        raise ValueError(f"{op}: A {tuple(a_shape)} and B {tuple(b_shape)} must be (rows, K) and (E, N, K)")
     a_dt = _operand_dtypes(A, B, op)
-    E, N, K = B.shape
+    E, N, K = b_shape
+    a_rows, kb = a_shape[0], _blocks(K)
     if _counts_of(counts, op) != E:
         raise ValueError(f"{op}: {counts.numel()} counts for {E} experts")
-    rows = A.shape[0] if row_sources is None else _sources_of(row_sources, op)
+    rows = a_rows if row_sources is None else _sources_of(row_sources, op)
     if rows > 1 << 24:
         raise ValueError(f"{op}: at most 2**24 expert rows")
-    if rows > 0 and A.shape[0] == 0:
+    if rows > 0 and a_rows == 0:
         raise ValueError(f"{op}: A has no rows")
-    lda, ldb = _values(A, "A", op), _values(B, "B", op)
-    if E > 1 and B.numel() and B.stride(0) % 16:
+    b_stride = B.stride()
+    lda, ldb = _values(A, a_rows, K, A.stride(), "A", op), _values(B, N, K, b_stride, "B", op)
+    if E > 1 and N and K and b_stride[0] % 16:
         raise ValueError(f"{op}: every expert's matrix must start at a 16-byte address")
-    sa_row, sa_k, _ = _scales(A_scales, A.shape[0], _blocks(K), False, "A_scales", op)
+    sa_row, sa_k, _ = _scales(A_scales, a_rows, kb, False, "A_scales", op)
     if B_scales.dim() != 3 or B_scales.shape[0] != E:
         raise ValueError(f"{op}: B_scales has shape {tuple(B_scales.shape)}, expected {E} experts")
-    sb_row, sb_k, b_tiles = _scales(B_scales, N, _blocks(K), True, "B_scales", op)
+    sb_row, sb_k, b_tiles = _scales(B_scales, N, kb, True, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, counts, row_sources, out, op=op)
-    D = _output(out, (rows, N), out_dtype, None, A.device, op)
+    D, d_dt, ldd, _, _, _ = _output(out, (rows, N), out_dtype, None, A.device, op)
     if rows == 0 or N == 0:
         return D
     with on_device(A):
-        rc = lib().fx_fp8_grouped_gemm(ptr(A), lda, a_dt, ptr(A_scales), sa_row, sa_k, ptr(row_sources), A.shape[0], ptr(B),
-                                       ldb, B.stride(0), ptr(B_scales), sb_row, sb_k, B_scales.stride(0), b_tiles,
-                                       ptr(counts), E, rows, ptr(D), _ld(D), N, K, dtype_enum(D.dtype), stream_ptr(A.device))
+        rc = lib().fx_fp8_grouped_gemm(A.data_ptr(), lda, a_dt, A_scales.data_ptr(), sa_row, sa_k,
+                                       None if row_sources is None else row_sources.data_ptr(), a_rows, B.data_ptr(), ldb,
+                                       b_stride[0], B_scales.data_ptr(), sb_row, sb_k, B_scales.stride(0), b_tiles,
+                                       counts.data_ptr(), E, rows, D.data_ptr(), ldd, N, K, d_dt, raw_stream(A))
     check(rc, "fx_fp8_grouped_gemm")
     return D
 
@@ -272,25 +304,27 @@ def flextrain_fp8_grouped_wgrad(A, A_scales, B, B_scales, counts, C=None, out=No
     ``A (M, capacity)`` e4m3 or e5m2, ``B (N, capacity)`` e4m3, scales ``(M | N, capacity / 128)``; ``out`` / ``C``
     ``(E, M, N)`` of one dtype (``C`` may be ``out``).  An expert without rows gives ``C[e]``, or zeros."""
     op = "flextrain_fp8_grouped_wgrad"
-    if A.dim() != 2 or B.dim() != 2 or A.shape[1] != B.shape[1]:
-        raise ValueError(f"{op}: A {tuple(A.shape)} and B {tuple(B.shape)} must be (M, capacity) and (N, capacity)")
+    a_shape, b_shape = A.shape, B.shape
+    if len(a_shape) != 2 or len(b_shape) != 2 or a_shape[1] != b_shape[1]:
+        raise ValueError(f"{op}: A {tuple(a_shape)} and B {tuple(b_shape)} must be (M, capacity) and (N, capacity)")
     a_dt = _operand_dtypes(A, B, op)
     E = _counts_of(counts, op)
-    (M, cap), N = A.shape, B.shape[0]
+    (M, cap), N = a_shape, b_shape[0]
     if cap % 128:
         raise ValueError(f"{op}: the capacity {cap} is not a multiple of 128")
-    if cap > 1 << 24:
-        raise ValueError(f"{op}: at most 2**24 expert rows")
-    lda, ldb = _values(A, "A", op), _values(B, "B", op)
+    if cap >= 1 << 23:
+        raise ValueError(f"{op}: at most 2**23 expert rows")
+    lda, ldb = _values(A, M, cap, A.stride(), "A", op), _values(B, N, cap, B.stride(), "B", op)
     sa_row, sa_k, _ = _scales(A_scales, M, cap // 128, False, "A_scales", op)
     sb_row, sb_k, _ = _scales(B_scales, N, cap // 128, False, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, counts, C, out, op=op)
-    D = _output(out, (E, M, N), out_dtype, C, A.device, op)
+    D, d_dt, ldd, d_batch, ldc, c_batch = _output(out, (E, M, N), out_dtype, C, A.device, op)
     if M == 0 or N == 0:
         return D
     with on_device(A):
-        rc = lib().fx_fp8_grouped_wgrad(ptr(A), lda, a_dt, ptr(A_scales), sa_row, sa_k, ptr(B), ldb, ptr(B_scales), sb_row, sb_k,
-                                        ptr(counts), E, cap, ptr(C), _ld(C), C.stride(0) if C is not None else 0, ptr(D), _ld(D),
-                                        D.stride(0), M, N, dtype_enum(D.dtype), stream_ptr(A.device))
+        rc = lib().fx_fp8_grouped_wgrad(A.data_ptr(), lda, a_dt, A_scales.data_ptr(), sa_row, sa_k, B.data_ptr(), ldb,
+                                        B_scales.data_ptr(), sb_row, sb_k, counts.data_ptr(), E, cap,
+                                        None if C is None else C.data_ptr(), ldc, c_batch, D.data_ptr(), ldd, d_batch, M, N,
+                                        d_dt, raw_stream(A))
     check(rc, "fx_fp8_grouped_wgrad")
     return D

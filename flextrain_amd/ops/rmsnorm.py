@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, require_gpu, require_same_device, stream_ptr
+from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, raw_stream, require_gpu, require_same_device, stream_ptr
 from .fp8 import _fp8_rows, _round_up, _scale_store, _blocks
 
 
@@ -148,24 +148,28 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     T, D, _, _ = _norm_config(X, W, None)
     if D == 0:
         raise ValueError(f"{op}: X has no columns")
-    for t, name in ((residual, "residual"), (sum_out, "sum_out")):
-        if t is not None:
-            _check_like(t, X, name)
+    if residual is not None:
+        _check_like(residual, X, "residual")
+    if sum_out is not None:
+        _check_like(sum_out, X, "sum_out")
     require_same_device(X, residual, W, sum_out, op=op)
-    x_dt = dtype_enum(X.dtype)
-    y_dt = x_dt if output_dtype is None or output_dtype == X.dtype else fp8_enum(output_dtype)
+    device, dtype = X.device, X.dtype
+    x_dt = dtype_enum(dtype)
+    y_dt = x_dt if output_dtype is None or output_dtype == dtype else fp8_enum(output_dtype)
     H = sum_out
     if H is None:
         H = torch.empty_like(X) if residual is not None else X
-    rstd = torch.empty(T, 1, dtype=torch.float32, device=X.device)
+    rstd = torch.empty((T, 1), dtype=torch.float32, device=device)
     if y_dt == x_dt:
         Y, scales, ldy = torch.empty_like(X), None, D
     else:
-        Y, scales, ldy = _fp8_rows((), T, D, output_dtype, X.device), _scale_store((), T, _blocks(D), X.device), _round_up(D, 16)
+        Y, scales = _fp8_rows(None, T, D, output_dtype, device), _scale_store(None, T, _blocks(D), device)
+        ldy = _round_up(D, 16)
     with on_device(X):
-        rc = lib().fx_add_rmsnorm_fwd(ptr(X), ptr(residual), ptr(W), ptr(H) if H is not X or residual is not None else None,
-                                      ptr(Y), ldy, ptr(scales), T, ptr(rstd), T, D, float(rms_norm_eps), x_dt,
-                                      dtype_enum(W.dtype) if W is not None else 0, y_dt, stream_ptr(X.device))
+        rc = lib().fx_add_rmsnorm_fwd(X.data_ptr(), None if residual is None else residual.data_ptr(),
+                                      None if W is None else W.data_ptr(), None if H is X and residual is None else H.data_ptr(),
+                                      Y.data_ptr(), ldy, None if scales is None else scales.data_ptr(), T, rstd.data_ptr(), T, D,
+                                      rms_norm_eps, x_dt, 0 if W is None else dtype_enum(W.dtype), y_dt, raw_stream(X))
     check(rc, "fx_add_rmsnorm_fwd")
     return Y, scales, H, rstd
 
@@ -205,6 +209,6 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
         rc = L.fx_add_rmsnorm_bwd(ptr(dY), ptr(dH), ptr(H), ptr(W), ptr(rstd), ptr(dX), ptr(dW),
                                   dtype_enum(dW.dtype) if dW is not None else 0, 1 if accumulate else 0, T, D,
                                   dtype_enum(H.dtype), dtype_enum(W.dtype) if W is not None else 0, ptr(ws), nbytes,
-                                  stream_ptr(H.device))
+                                  raw_stream(H))
     check(rc, "fx_add_rmsnorm_bwd")
     return dX, dW
