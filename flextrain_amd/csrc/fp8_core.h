@@ -17,6 +17,9 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int FP8_BK = 128;
 
+// The compiler sees a new value (no instruction): what is computed from it stays where it is written.
+#define FX_OPAQUE(x) asm volatile("" : "+v"(x))
+
 // A wave-uniform pointer to global memory held in scalar registers (a no-op where the compiler knows).
 typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
 FX_DEV global_bytes uniform_ptr(const uint8_t* p) {
@@ -88,6 +91,7 @@ struct Fp8Loop {
     int rawa[TM / 2], rawb;               // scale bytes requested for the next K-step
     int sca, scb;                         // packed scales of the current one
     int wave, lane;
+    unsigned lds_lane;
 
     // source row of tile row r of A (clamped to the last one; its products are never stored)
     static FX_DEV int64_t a_row(const Fp8Job<TD>& j, int r) {
@@ -107,12 +111,19 @@ struct Fp8Loop {
             if (IDX == LD - 1) bbase += FP8_BK;
         }
     }
+    FX_DEV void move(int bytes) { abase += bytes; bbase += bytes; }
     FX_DEV void issue(uint8_t* buf) { static_for<0, LD>([&](auto i) { issue_one<decltype(i)::value>(buf); }); }
 
     FX_DEV void fetch_scales() {
 #pragma unroll
-        for (int i = 0; i < TM / 2; ++i) rawa[i] = uniform_ptr(sabase)[soa[i]];
-        rawb = uniform_ptr(sbbase)[sob];
+        for (int i = 0; i < TM / 2; ++i) {
+            unsigned o = soa[i];
+            FX_OPAQUE(o);             // a 32-bit offset here, not a 64-bit one kept in a register pair
+            rawa[i] = uniform_ptr(sabase)[o];
+        }
+        unsigned o = sob;
+        FX_OPAQUE(o);
+        rawb = uniform_ptr(sbbase)[o];
         sabase += sak;
         sbbase += sbk;
     }
@@ -128,10 +139,45 @@ struct Fp8Loop {
         b = (int)(y[0] | (y[1] << 8));
     }
 
-    // Set up the tile and request its first K-step into buf0.
-    FX_DEV void begin(const Fp8Job<TD>& j, uint8_t* buf0) {
+    FX_DEV void init() {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int r = lane & 31, h = lane >> 5;
+        lds_lane = (unsigned)(r * FP8_BK + (((2 * h) ^ swz(r)) << 4));
+    }
+
+    // A contraction (K = 0 mod 128, or K > 128) is walked in steps(K) >= 2 K-steps.  When K is no multiple of 128 the last
+    // step starts back(K) bytes early, so that it ends where the row's last 16-byte chunk ends and no load leaves the
+    // row; patch() then zeroes the bytes that belong to the step before and those behind K.  A contraction of 128 has a
+    // second step made of such bytes only.
+    static FX_DEV int steps(int K) { return max(2, (K + FP8_BK - 1) / FP8_BK); }
+    static FX_DEV int back(int K) { return steps(K) * FP8_BK - ((K + 15) & ~15); }
+    // Zero what lies outside bytes [lo, hi) of the landed K-step in `buf`: every lane mends the chunks it loaded itself (its
+    // loads have been waited for; a barrier follows).  lo is a multiple of 16.
+    FX_DEV void patch(uint8_t* buf, int lo, int hi) const {
+        const int rr = lane >> 3, pos = lane & 7;
+#pragma unroll 1
+        for (int i = 0; i < NA + NB; ++i) {
+            const bool is_a = i < NA;
+            const int q = (is_a ? i : i - NA) * NW + wave;
+            const int c = pos ^ swz(q * 8 + rr);
+            if (c * 16 < lo || c * 16 + 16 > hi) {
+                uint8_t* p = buf + (is_a ? 0 : BM * FP8_BK) + q * 1024 + lane * 16;
+                u32x4_t x = *reinterpret_cast<const u32x4_t*>(p);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const int left = c * 16 < lo ? 0 : hi - c * 16 - d * 4;          // bytes of this word that stay
+                    x[d] = left >= 4 ? x[d] : left <= 0 ? 0u : x[d] & (0xffffffffu >> (8 * (4 - left)));
+                }
+                *reinterpret_cast<u32x4_t*>(p) = x;
+            }
+        }
+    }
+
+    // Loads and scales of tile j (K > 0) from here on.
+    FX_DEV void setup(const Fp8Job<TD>& j) {
+        int lane = this->lane;
+        FX_OPAQUE(lane);          // keeps the pieces of the offsets from being carried through the K loop in registers
         const int wm = wave / WAVES_N, wn = wave % WAVES_N;
         const int rr = lane >> 3, pos = lane & 7;
         const bool gathered = j.row_map != nullptr;
@@ -154,20 +200,29 @@ struct Fp8Loop {
         sob = (unsigned)(min(j.n0 + wn * WN + lane, j.B.ext - 1) >> j.B.s_shift) * (unsigned)j.B.s_row;
         sabase = j.A.s;
         sbbase = j.B.s;
-        sak = j.A.s_k;
-        sbk = j.B.s_k;
-        if (j.K >= FP8_BK) issue(buf0);
-        if (j.K > 0) fetch_scales();
+        sak = j.K > FP8_BK ? j.A.s_k : 0;         // (a contraction of one block has one scale)
+        sbk = j.K > FP8_BK ? j.B.s_k : 0;
     }
 
-    // The 32 k-values of this lane in tile row row0 + (lane & 31), sub-step ks.
+    // First tile of a workgroup: its first two K-steps requested, the first landed and readable by everyone.
+    FX_DEV void start(const Fp8Job<TD>& j, uint8_t* buf0, uint8_t* buf1) {
+        setup(j);
+        fetch_scales();
+        issue(buf0);
+        move(steps(j.K) == 2 ? -back(j.K) : 0);
+        issue(buf1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LD) : "memory");
+        __syncthreads();
+    }
+
+    // The 32 k-values of this lane in tile row row0 + (lane & 31), sub-step ks: chunks c = 4 ks + 2 h and c + 1 of that row,
+    // at positions c ^ swz(row).  lds_lane is the byte offset of chunk 2 h; the others differ from it in bits 4 and 6.
+    // (row0 is a multiple of 32: swz(row0 + r) = swz(r).)
     FX_DEV i32x8_t read_frag(const uint8_t* tile, int row0, int ks) const {
-        const int r = lane & 31, h = lane >> 5, s = swz(r);        // row0 is a multiple of 32: swz(row0 + r) = swz(r)
-        const uint8_t* p = tile + (row0 + r) * FP8_BK;
-        const int c = ks * 4 + h * 2;
         union { i32x8_t f; u32x4_t q[2]; } u;
-        u.q[0] = *reinterpret_cast<const u32x4_t*>(p + ((c ^ s) << 4));
-        u.q[1] = *reinterpret_cast<const u32x4_t*>(p + (((c + 1) ^ s) << 4));
+        const unsigned o = lds_lane ^ (unsigned)(ks * 64);
+        u.q[0] = *reinterpret_cast<const u32x4_t*>(tile + row0 * FP8_BK + o);
+        u.q[1] = *reinterpret_cast<const u32x4_t*>(tile + row0 * FP8_BK + (o ^ 16u));
         return u.f;
     }
     template <int I, int P>
@@ -214,16 +269,18 @@ struct Fp8Loop {
     }
     struct Nothing { template <typename I> FX_DEV void operator()(I) const {} };
 
-    // One K-step from `cur` whose successor is in (or on its way to) `nxt`; with MORE the one after that is requested
-    // into `cur`.
-    template <bool MORE>
-    FX_DEV void step(f32x16_t (&acc)[TM][TN], uint8_t* cur, uint8_t* nxt) {
-        fetch_scales();                                  // of the next K-step; they land with its tiles below
+    // One K-step from `cur` whose successor, of which bytes [lo, hi) count, is in (or on its way to) `nxt`; the caller has called
+    // fetch_scales() for the successor.  With MORE the K-step that the loader stands at is requested into `cur`.
+    template <bool MORE, bool SHORT>
+    FX_DEV void step(f32x16_t (&acc)[TM][TN], uint8_t* cur, uint8_t* nxt, int lo, int hi) {
         sub<0, true>(acc, cur, 1, Nothing());
         // every read of `cur` is out.  Once they and this wave's loads into `nxt` have landed, the barrier makes `nxt`
         // readable and `cur` writable for everyone; the second half's MFMAs run after it, while the first fragments
         // of the next K-step are read and the loads of the one after go out.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (SHORT) {
+            if (lo > 0) patch(nxt, lo, hi);
+        }
         __syncthreads();
         // packed here, where nothing is in flight: a use further down would wait for the tile loads issued since
         int na, nb;
@@ -235,10 +292,28 @@ struct Fp8Loop {
         sca = na;
         scb = nb;
     }
+    // The last K-step; with MORE the next tile's second K-step goes into `cur` once everyone has read it.
+    template <bool MORE>
+    FX_DEV void last_step(f32x16_t (&acc)[TM][TN], uint8_t* cur) {
+        sub<0, true>(acc, cur, 1, Nothing());
+        if constexpr (MORE) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        sub<1, false>(acc, cur, 0, [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            if constexpr (MORE) static_for<M * PER, (M + 1) * PER>([&](auto i) { issue_one<decltype(i)::value>(cur); });
+        });
+    }
 
-    // K loop; leaves the (transposed) accumulators of this wave's sub-tile and ends with a barrier.
-    // first_landed: the loads of K-step 0 have been waited for, with a barrier since.
-    FX_DEV void finish(const Fp8Job<TD>& job, uint8_t* buf0, uint8_t* buf1, f32x16_t (&acc)[TM][TN], bool first_landed) {
+    // K loop of tile `job` (K > 0), whose first K-step is readable in buf[par] and whose second is landed in or on its way
+    // to buf[1 - par], scales of the first requested.  Leaves the (transposed) accumulators.
+    // AHEAD: the stages go on without a gap into tile `next`: its first K-step is requested while the last but one of this
+    // tile is multiplied, its second during the last, so both arrive under MFMAs and the epilogue; par moves on to where
+    // its first K-step is.  (Behind a workgroup's last tile `next` is that tile again: a condition around MFMAs
+    // would cost registers, two K-steps fetched for nothing cost nothing.)
+    template <bool AHEAD>
+    FX_DEV void run(const Fp8Job<TD>& job, const Fp8Job<TD>& next, uint8_t* buf0, uint8_t* buf1, int& par, f32x16_t (&acc)[TM][TN]) {
         const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -246,127 +321,238 @@ struct Fp8Loop {
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
-        const int K = job.K, nfull = K / FP8_BK;
+        const int K = job.K, n = steps(K);
+        const int lo = back(K), hi = lo + K - (n - 1) * FP8_BK;         // what counts of the last step
         // wave-uniform: does any element of this wave's sub-tile exist?
         const bool live = __builtin_amdgcn_readfirstlane((job.m0 + wm * WM < job.A.ext) && (job.n0 + wn * WN < job.B.ext));
-        auto stage = [&](int kt) { return (kt & 1) ? buf1 : buf0; };
-        if (nfull > 0) {
-            if (nfull > 1) issue(buf1);
-            if (!first_landed) {
-                if (nfull > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LD) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const int p0 = par;
+        par = (p0 + n) & 1;
+        auto stage = [&](int kt) { return ((kt + p0) & 1) ? buf1 : buf0; };
+        const int next_back = steps(next.K) == 2 ? back(next.K) : 0;
+        if (live) {
+            pack_scales(sca, scb);
+            static_for<0, TN>([&](auto j) { read_b<decltype(j)::value, 0>(stage(0), 0); });
+            static_for<0, TM>([&](auto i) { read_a<decltype(i)::value, 0>(stage(0), 0); });
+            // straight-line K-steps: a branch between the MFMAs lets the compiler sink them all behind the loads
+            for (int kt = 0; kt < n - 2; ++kt) {
+                move(kt == n - 3 ? -lo : 0);
+                fetch_scales();
+                step<true, false>(acc, stage(kt), stage(kt + 1), 0, FP8_BK);
+            }
+            fetch_scales();
+            if (AHEAD) setup(next);
+            step<AHEAD, true>(acc, stage(n - 2), stage(n - 1), lo, hi);
+            if (AHEAD) { move(-next_back); fetch_scales(); }
+            last_step<AHEAD>(acc, stage(n - 1));
+        } else {
+            // this wave loads its share of the stages, meets every barrier of the other branch and leaves the matrix
+            // pipe to the wave it shares a SIMD with
+            for (int kt = 0; kt < n - 2; ++kt) {
+                move(kt == n - 3 ? -lo : 0);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
+                issue(stage(kt));
             }
-            if (!live) {
-                // this wave keeps loading its share of the stages, meets every barrier of the loop below and leaves
-                // the matrix pipe to the wave it shares a SIMD with
-                for (int kt = 0; kt + 1 < nfull; ++kt) {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                    __syncthreads();
-                    if (kt + 2 < nfull) issue(stage(kt));
-                }
-            } else {
-                pack_scales(sca, scb);
-                static_for<0, TN>([&](auto j) { read_b<decltype(j)::value, 0>(buf0, 0); });
-                static_for<0, TM>([&](auto i) { read_a<decltype(i)::value, 0>(buf0, 0); });
-                // straight-line K-steps: a branch between the MFMAs lets the compiler sink them all behind the loads
-                for (int kt = 0; kt + 2 < nfull; ++kt) step<true>(acc, stage(kt), stage(kt + 1));
-                if (nfull > 1) step<false>(acc, stage(nfull - 2), stage(nfull - 1));
-                uint8_t* cur = stage(nfull - 1);
-                sub<0, true>(acc, cur, 1, Nothing());
-                sub<1, false>(acc, cur, 0, Nothing());
-            }
-        }
-        if (nfull * FP8_BK < K) {
-            // last partial K-step: through registers, zero behind K.  `buf` was last read two K-steps ago.
-            uint8_t* buf = stage(nfull);
-            const int tid = threadIdx.x;
-            if (nfull > 0) fetch_scales();       // (with no full K-step begin() has requested these)
-            for (int id = tid; id < (BM + BN) * 8; id += NT) {
-                const int r = id >> 3, c = id & 7, k = nfull * FP8_BK + c * 16;
-                const uint8_t* row = r < BM ? job.A.p + a_row(job, r) * job.A.ld
-                                            : job.B.p + (int64_t)min(job.n0 + r - BM, job.B.ext - 1) * job.B.ld;
-                const u32x4_t v = load_chunk(row, k, K);
-                *reinterpret_cast<u32x4_t*>(buf + r * FP8_BK + ((c ^ swz(r)) << 4)) = v;
-            }
+            if (AHEAD) setup(next);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (lo > 0) patch(stage(n - 1), lo, hi);
             __syncthreads();
-            if (live) {
-                pack_scales(sca, scb);
-                static_for<0, TN>([&](auto j) { read_b<decltype(j)::value, 0>(buf, 0); });
-                static_for<0, TM>([&](auto i) { read_a<decltype(i)::value, 0>(buf, 0); });
-                sub<0, true>(acc, buf, 1, Nothing());
-                sub<1, false>(acc, buf, 0, Nothing());
+            if (AHEAD) {
+                issue(stage(n - 2));
+                move(-next_back);
+                fetch_scales();
+                __syncthreads();
+                issue(stage(n - 1));
             }
         }
-        __syncthreads();      // every wave is past its last LDS read: the stages are free
     }
 };
+
+// D (+ C) of one wave from its accumulators, straight from registers.  Lane (r, h) = (lane % 32, lane / 32) holds of row
+// 32 i + r the columns 32 j + 8 g + 4 h .. + 3 (g = 0 .. 3): swapping the upper half-wave of group 2 q with the lower one
+// of group 2 q + 1 leaves it 8 consecutive columns, 16 bytes of a 2-byte type.  Staging the tile through LDS instead (full
+// 256-byte runs per store) cost 33,000 cycles per 256 x 256 tile, half the K loop of a 2048-long contraction.
+// LAND: before the first store, everything this wave has requested so far must have landed (loads and stores share one
+// counter: a wait placed after the stores would also wait for them to drain).
+template <typename TD, int TM, int TN, bool LAND>
+FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc, TD* D, int64_t ldd, int row_base, int col_base,
+                         int M, int N, int lane) {
+    typedef typename VecOf<TD>::type Pack;
+    constexpr int PN = 8 / VecOf<TD>::N;                     // 16-byte packs of 8 columns
+    constexpr int CB = PN == 1 ? TM : (TM + 1) / 2;          // row bands whose C is requested together
+    const int r = lane & 31, h = lane >> 5;
+    const bool vec = (ldd % VecOf<TD>::N) == 0 && (reinterpret_cast<uintptr_t>(D) & 15u) == 0 &&
+                     (C == nullptr || ((ldc % VecOf<TD>::N) == 0 && (reinterpret_cast<uintptr_t>(C) & 15u) == 0));
+    // wave-uniform: every row and column of this wave exists
+    const bool full = vec && row_base + 32 * TM <= M && col_base + 32 * TN <= N;
+    auto gather = [&](int i, int j, int q, float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float lo = acc[i][j][8 * q + e], hi = acc[i][j][8 * q + 4 + e];
+            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+            v[e] = __builtin_bit_cast(float, (unsigned)x[0]);
+            v[4 + e] = __builtin_bit_cast(float, (unsigned)x[1]);
+        }
+    };
+    if (full && C == nullptr) {
+        if (LAND) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        TD* d0 = D + (int64_t)(row_base + r) * ldd + col_base + h * 8;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float v[8];
+                    gather(i, j, q, v);
+                    store_f32<TD, 8>(d0 + (int64_t)i * 32 * ldd + j * 32 + q * 16, v);
+                }
+    } else if (full) {
+        Pack c[CB][TN][2][PN];
+        const TD* c0 = C + (int64_t)(row_base + r) * ldc + col_base + h * 8;
+        TD* d0 = D + (int64_t)(row_base + r) * ldd + col_base + h * 8;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            if (i % CB == 0) {
+#pragma unroll
+                for (int b = 0; b < CB; ++b)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+#pragma unroll
+                            for (int u = 0; u < PN; ++u)
+                                c[b][j][q][u] = *reinterpret_cast<const Pack*>(c0 + (int64_t)(i + b) * 32 * ldc + j * 32 + q * 16 + u * VecOf<TD>::N);
+                if (LAND && i == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float v[8];
+                    gather(i, j, q, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += (float)c[i % CB][j][q][e / VecOf<TD>::N][e % VecOf<TD>::N];
+                    store_f32<TD, 8>(d0 + (int64_t)i * 32 * ldd + j * 32 + q * 16, v);
+                }
+        }
+    } else {
+        if (LAND) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    float v[8];
+                    gather(i, j, q, v);
+                    const int row = row_base + i * 32 + r, col = col_base + j * 32 + q * 16 + h * 8;
+                    if (row >= M || col >= N) continue;
+                    TD* d = D + (int64_t)row * ldd + col;
+                    if (vec && col + 8 <= N) {
+                        if (C != nullptr) {
+                            float add[8];
+                            load_f32<TD, 8>(C + (int64_t)row * ldc + col, add);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] += add[e];
+                        }
+                        store_f32<TD, 8>(d, v);
+                    } else {
+                        for (int e = 0; e < 8 && col + e < N; ++e) {
+                            float o = v[e];
+                            if (C != nullptr) o += (float)C[(int64_t)row * ldc + col + e];
+                            d[e] = (TD)o;
+                        }
+                    }
+                }
+    }
+}
 
 // ---------------------------------------------------------------- kernels over a list of tiles
 // A Source names the tiles of a launch: total(lane) how many there are, locate(id, lane) where tile `id` lies (a small
 // struct), job(where) its operands.  Counts of experts are read by whole waves (find_group_tile), so every lane calls.
 
-// 256 x 256 tiles, eight waves of 128 x 64, one workgroup per CU that walks the list with the grid as stride: the first
-// K-step of its next tile is requested before the epilogue of the current one.
-// LDS: [stage 0: 64 KB][stage 1: 64 KB, and the epilogue's staging, which reaches 4 KB past it]; the staging may
-// overlap stage 1 because the second K-step of the next tile is issued after the barrier behind the epilogue.
+// 256 x 256 tiles, eight waves of 128 x 64, one workgroup per CU that walks the list with the grid as stride (Fp8Loop::run
+// keeps its loads going over the tile boundaries).  LDS: two stages of 64 KB.
 constexpr int FP8_WALK_BM = 256, FP8_WALK_BN = 256;
-constexpr size_t kFp8WalkLds = 64 * 1024 + epilogue_lds_bytes<8, 64>();
+constexpr size_t kFp8WalkLds = 128 * 1024;
 
-template <int AF, typename TD, bool NT, typename Source>
+// A tile whose contraction is empty: C, or zeros.
+template <typename TD, int BM, int BN, int NT>
+FX_DEV void fp8_empty_tile(const Fp8Job<TD>& j, int64_t ldc, int64_t ldd) {
+    const int rows = min(BM, j.A.ext - j.m0), cols = min(BN, j.B.ext - j.n0);
+    for (int r = threadIdx.x / 64; r < rows; r += NT / 64)
+        for (int c = threadIdx.x % 64; c < cols; c += 64) {
+            const int64_t m = j.m0 + r, n = j.n0 + c;
+            j.D[m * ldd + n] = j.C != nullptr ? j.C[m * ldc + n] : (TD)0.f;
+        }
+}
+
+template <int AF, typename TD, typename Source>
 __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
     extern __shared__ __align__(16) unsigned char smem[];
     typedef Fp8Loop<AF, TD, FP8_WALK_BM, FP8_WALK_BN, 2, 4> Loop;
-    static_assert(Loop::STAGE == 64 * 1024, "the LDS plan assumes 64 KB stages");
+    static_assert(2 * Loop::STAGE == (int)kFp8WalkLds, "two stages");
     uint8_t *buf0 = smem, *buf1 = smem + Loop::STAGE;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int total = src.total(lane);
-    int id = blockIdx.x;
-    if (id >= total) return;
     Loop loop;
-    auto cur = src.locate(id, total, lane);
-    loop.begin(src.job(cur), buf0);
-    bool landed = false;
+    loop.init();
+    const int total = src.total(loop.lane);
+    // the next tile from `id` on that has a contraction; those without are written on the way
+    auto find = [&](int& id, typename Source::Where& w) {
+        for (; id < total; id += (int)gridDim.x) {
+            w = src.locate(id, total, loop.lane);
+            const Fp8Job<TD> j = src.job(w);
+            if (j.K > 0) return true;
+            fp8_empty_tile<TD, FP8_WALK_BM, FP8_WALK_BN, 512>(j, src.ldc, src.ldd);
+        }
+        return false;
+    };
+    int id = blockIdx.x;
+    typename Source::Where cur;
+    if (!find(id, cur)) return;
+    loop.start(src.job(cur), buf0, buf1);
+    int par = 0;
     for (;;) {
-        const int next = id + (int)gridDim.x;
-        const bool more = next < total;
-        auto nxt = cur;
-        if (more) nxt = src.locate(next, total, lane);
+        typename Source::Where nxt = cur;
+        id += (int)gridDim.x;
+        const bool more = find(id, nxt);
+        if (!more) nxt = cur;
         f32x16_t acc[Loop::TM][Loop::TN];
-        loop.finish(src.job(cur), buf0, buf1, acc, landed);
-        if (more) loop.begin(src.job(nxt), buf0);
+        loop.template run<true>(src.job(cur), src.job(nxt), buf0, buf1, par, acc);
         const Fp8Job<TD> j = src.job(cur);
-        epilogue_tile<bf16, TD, Loop::WM, Loop::WN, true, NT>(acc, j.C, j.D, src.ldc, src.ldd, j.m0 + (wave / 4) * Loop::WM,
-                                                              j.n0 + (wave % 4) * Loop::WN, j.A.ext, j.B.ext, 1.f, j.C != nullptr ? 1.f : 0.f,
-                                                              reinterpret_cast<bf16*>(buf1), wave, lane);
+        fp8_epilogue<TD, Loop::TM, Loop::TN, true>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 4) * Loop::WM,
+                                                   j.n0 + (loop.wave % 4) * Loop::WN, j.A.ext, j.B.ext, loop.lane);
         if (!more) break;
-        __syncthreads();
-        landed = true;
+        __syncthreads();          // everyone's share of the next tile's first K-steps has landed
         cur = nxt;
-        id = next;
     }
 }
 
 // 128 x 128 tiles, four waves of 64 x 64, one tile per workgroup; 64 KB of LDS, so two workgroups share a CU and one's
 // epilogue and first loads run under the other's K loop.
+constexpr size_t kFp8Tile128Lds = 64 * 1024;
+
 template <int AF, typename TD, typename Source>
 __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
     extern __shared__ __align__(16) unsigned char smem[];
     typedef Fp8Loop<AF, TD, 128, 128, 2, 2> Loop;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int total = src.total(lane);
-    if ((int)blockIdx.x >= total) return;
+    static_assert(2 * Loop::STAGE == (int)kFp8Tile128Lds, "two stages");
     Loop loop;
-    const Fp8Job<TD> j = src.job(src.locate(blockIdx.x, total, lane));
-    loop.begin(j, smem);
+    loop.init();
+    const int total = src.total(loop.lane);
+    if ((int)blockIdx.x >= total) return;
+    const Fp8Job<TD> j = src.job(src.locate(blockIdx.x, total, loop.lane));
+    if (j.K == 0) {
+        fp8_empty_tile<TD, 128, 128, 256>(j, src.ldc, src.ldd);
+        return;
+    }
+    loop.start(j, smem, smem + Loop::STAGE);
     f32x16_t acc[Loop::TM][Loop::TN];
-    loop.finish(j, smem, smem + Loop::STAGE, acc, false);
-    epilogue_tile<bf16, TD, Loop::WM, Loop::WN>(acc, j.C, j.D, src.ldc, src.ldd, j.m0 + (wave / 2) * Loop::WM,
-                                                j.n0 + (wave % 2) * Loop::WN, j.A.ext, j.B.ext, 1.f, j.C != nullptr ? 1.f : 0.f,
-                                                reinterpret_cast<bf16*>(smem), wave, lane);
+    int par = 0;
+    loop.template run<false>(j, j, smem, smem + Loop::STAGE, par, acc);
+    fp8_epilogue<TD, Loop::TM, Loop::TN, false>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 2) * Loop::WM,
+                                                j.n0 + (loop.wave % 2) * Loop::WN, j.A.ext, j.B.ext, loop.lane);
 }
-constexpr size_t kFp8Tile128Lds = 64 * 1024;
-static_assert(epilogue_lds_bytes<4, 64>() <= kFp8Tile128Lds, "epilogue staging");
 
 // Small products: one workgroup per tile of 16 MT x 16 NT, its NW waves share the contraction (wave w takes K-steps
 // w, w + NW, ..) and add up through LDS in ascending order.  Operands go straight from memory into registers: with

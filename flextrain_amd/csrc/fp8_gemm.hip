@@ -47,7 +47,7 @@ struct Fp8Split {
     FX_DEV Fp8Job<float> job(const Where& w) const {
         Fp8Job<float> j{A, B, w.m0, w.n0, 0, nullptr, 0, nullptr, P + (int64_t)w.split * A.ext * B.ext};
         const int k0 = w.split * k_slice;
-        j.K = min(k_slice, K - k0);
+        j.K = w.split == splits - 1 ? K - k0 : k_slice;
         j.A.p += k0;
         j.B.p += k0;
         j.A.s += (int64_t)(k0 / FP8_BK) * A.s_k;
@@ -77,7 +77,7 @@ struct Fp8Plan { int tile, splits, k_slice; };      // tile 256 or 128; 16, 32, 
 static Fp8Plan fp8_plan(int M, int N, int K) {
     if (M <= 16) return Fp8Plan{16, 1, K};
     if (M <= 32) return Fp8Plan{32, 1, K};
-    if (M <= 64) return Fp8Plan{64, 1, K};
+    if (M <= 64 || K < FP8_BK) return Fp8Plan{64, 1, K};       // (the tile loads want a whole block)
     const int64_t big = (int64_t)fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
     if (big >= 192) return Fp8Plan{256, 1, K};
     const int64_t small = (int64_t)fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
@@ -89,8 +89,10 @@ static Fp8Plan fp8_plan(int M, int N, int K) {
         if (splits > 16) splits = 16;
         if (splits < 1) splits = 1;
     }
-    const int per = fp8_cdiv(steps, splits);
-    return Fp8Plan{128, fp8_cdiv(steps, per > 0 ? per : 1), per * FP8_BK};
+    const int slice = fp8_cdiv(steps, splits) * FP8_BK;
+    splits = fp8_cdiv(K, slice);
+    if (splits > 1 && K - (splits - 1) * slice < FP8_BK) --splits;      // the last slice takes what is short of a block
+    return Fp8Plan{128, splits, slice};
 }
 
 template <int AF, typename TD>
@@ -101,7 +103,7 @@ static int launch_dense(const Fp8View& a, const Fp8View& b, const TD* C, int64_t
         const Fp8Dense<TD, 256, 256> src{a, b, C, D, ldc, ldd, K, fp8_cdiv(M, 256), fp8_cdiv(N, 256)};
         const int64_t total = (int64_t)src.tiles_m * src.tiles_n;
         const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, false, Fp8Dense<TD, 256, 256>>;
+        auto kern = fp8_walk_kernel<AF, TD, Fp8Dense<TD, 256, 256>>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
         kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
         FX_CHECK_LAUNCH("fx_fp8_gemm");

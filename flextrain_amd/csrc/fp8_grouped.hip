@@ -71,7 +71,8 @@ struct Fp8GroupedWgrad {
 
 // Tile rows (their logarithm): 256 when experts average 384 rows or more, 128 (two workgroups per CU), and the small
 // kernel's 64, 32 or 16 when they average fewer than that.
-static int fp8_rows_shift(int64_t total_rows, int E) {
+static int fp8_rows_shift(int64_t total_rows, int E, int K) {
+    if (K < FP8_BK) return 6;                    // (the tile loads want a whole block)
     const int64_t avg = total_rows / E;
     return avg >= 384 ? 8 : avg >= 64 ? 7 : avg >= 32 ? 6 : avg >= 16 ? 5 : 4;
 }
@@ -80,7 +81,7 @@ template <int AF, typename TD>
 static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int64_t sb_expert, const int32_t* counts,
                        const int32_t* map, int64_t a_rows, TD* D, int64_t ldd, int64_t total_rows, int E, int K, hipStream_t stream) {
     const int N = b.ext;
-    const int shift = fp8_rows_shift(total_rows, E);
+    const int shift = fp8_rows_shift(total_rows, E, K);
     // at most this many row tiles, whatever the split over the experts
     const int64_t most = (total_rows >> shift) + (E < total_rows ? E : total_rows);
     const int tiles_n = fp8_cdiv(N, shift >= 7 ? 1 << shift : shift == 4 ? 16 : 32);
@@ -89,7 +90,7 @@ static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int
         typedef Fp8GroupedRows<TD, 8, 256> Source;
         const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};
         const unsigned grid = (unsigned)(most * tiles_n < fp8_walk_grid() ? most * tiles_n : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        auto kern = fp8_walk_kernel<AF, TD, Source>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
         kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
 #define FX_SMALL(SHIFT, MT, NT, NW, U)                                                                       \
@@ -122,7 +123,7 @@ static int launch_wgrad(const Fp8View& a, const Fp8View& b, const int32_t* count
         typedef Fp8GroupedWgrad<TD, 256, 256> Source;
         const Source src{a, b, counts, C, D, ldc, ldd, c_expert, d_expert, capacity, E, fp8_cdiv(M, 256), fp8_cdiv(N, 256)};
         const unsigned grid = (unsigned)(big < fp8_walk_grid() ? big : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        auto kern = fp8_walk_kernel<AF, TD, Source>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
         kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
     } else {

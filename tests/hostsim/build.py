@@ -109,6 +109,8 @@ def rewrite_asm(text):
             return "hostsim::lds_dma16(lds_addr, gptr);"
         if "global_load_lds_dwordx4 %1, %2" in body:
             return "hostsim::lds_dma16(lds_addr, reinterpret_cast<const char*>(sbase) + lane_off);"
+        if body.startswith('""'):                 # an empty statement that only hides a value from the compiler
+            return "((void)0)" + (";" if m.group(0).endswith(";") else "")
         assert "s_waitcnt" in body, f"inline assembly the host simulation has no stand-in for: {body[:80]}"
         count = re.search(r"vmcnt\((\d+|%0)\)", body)
         if count is None:
