@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
             unsigned m = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = max(m, finite_mag(y[j]));
-            const int b = scale_byte<OUT>(group_umax<16>(m));
+            const int b = scale_byte<OUT>(row16_umax(m));
             const float inv = inverse_scale(b);
             if (row_ok && col < ldy) {
                 uint2 o;

@@ -65,6 +65,92 @@ FX_DEV unsigned group_umax(unsigned v) {
     return v;
 }
 
+// Largest of the 16 lanes of a row of the wave (rotations within the row: no LDS round trips), and of the four rows.
+FX_DEV unsigned row16_umax(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));     // row_ror:8
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+}
+FX_DEV unsigned rows4_umax(unsigned v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);      // rows 0 and 2 twice / rows 1 and 3 twice
+    v = max((unsigned)a[0], (unsigned)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((unsigned)b[0], (unsigned)b[1]);
+}
+
+// ---------------------------------------------------------------- 2-byte inputs, two to a register
+// Magnitudes of bf16 / fp16 values order like their low 15 bits, so maxima are taken on pairs as they come from memory, and
+// v_cvt_scalef32_pk_{fp8,bf8}_{bf16,f16} divides a pair by its scale and rounds it in one instruction (checked over all
+// 65,536 inputs of either type: nearest even, subnormals kept).
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+
+FX_DEV unsigned pk_umax(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+template <typename T> struct Half;
+template <> struct Half<bf16> {
+    static constexpr unsigned INF = 0x7f80u;                 // magnitude bits from here on are not finite
+    static FX_DEV unsigned f32_bits(unsigned m) { return m << 16; }
+};
+template <> struct Half<f16> {
+    static constexpr unsigned INF = 0x7c00u;
+    static FX_DEV unsigned f32_bits(unsigned m) {
+        const unsigned short h = (unsigned short)m;
+        const float f = (float)__builtin_bit_cast(f16, h);
+        return __builtin_bit_cast(unsigned, f);
+    }
+};
+// Magnitude bits of a pair, 0 in the place of a value that is not finite.
+template <typename T>
+FX_DEV unsigned pk_finite(unsigned x) {
+    unsigned lo = x & 0x7fffu, hi = (x >> 16) & 0x7fffu;
+    lo = lo < Half<T>::INF ? lo : 0u;
+    hi = hi < Half<T>::INF ? hi : 0u;
+    return lo | (hi << 16);
+}
+// Two pairs, divided by 2^(byte - 127), to four bytes.
+template <typename T, int FMT>
+FX_DEV unsigned cvt_pairs(unsigned p0, unsigned p1, int byte) {
+    const unsigned sb = (unsigned)byte << 23;
+    const float scale = __builtin_bit_cast(float, sb);
+    s16x2_t w = {0, 0};
+    typedef T pair_t __attribute__((ext_vector_type(2)));
+    const pair_t a = __builtin_bit_cast(pair_t, p0), b = __builtin_bit_cast(pair_t, p1);
+    if constexpr (__is_same(T, bf16) && FMT == DT_E4M3) {
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, a, scale, false);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, b, scale, true);
+    } else if constexpr (__is_same(T, bf16)) {
+        w = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(w, a, scale, false);
+        w = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(w, b, scale, true);
+    } else if constexpr (FMT == DT_E4M3) {
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, a, scale, false);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, b, scale, true);
+    } else {
+        w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(w, a, scale, false);
+        w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(w, b, scale, true);
+    }
+    return __builtin_bit_cast(unsigned, w);
+}
+// Eight consecutive 2-byte values of a row as four pairs, 0 behind its end.
+template <typename T, bool VEC>
+FX_DEV void load4_pairs(const T* row, int64_t col, int64_t cols, unsigned (&o)[4]) {
+    if (VEC && col < cols) {
+        typedef unsigned u4_t __attribute__((ext_vector_type(4)));
+        const u4_t v = *reinterpret_cast<const u4_t*>(row + col);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = v[d];
+    } else {
+        const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const unsigned lo = !VEC && col + 2 * d < cols ? p[col + 2 * d] : 0u, hi = !VEC && col + 2 * d + 1 < cols ? p[col + 2 * d + 1] : 0u;
+            o[d] = lo | (hi << 16);
+        }
+    }
+}
+
 // Eight consecutive values of a row that has `cols` of them, 0 behind its end.  VEC: the address is 16-byte
 // aligned and a pack never straddles the end.
 template <typename T, bool VEC, bool NT = false>
@@ -87,23 +173,28 @@ FX_DEV void load8_or_zero(const T* row, int64_t col, int64_t cols, float (&o)[8]
 // A value that all lanes hold alike, in a scalar register.
 FX_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-FX_DEV int wave_scan(int v, int lane) {          // inclusive
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const int a = __shfl_up(v, off, 64);
-        if (lane >= off) v += a;
-    }
+// Inclusive sum over the lanes of a wave: within rows of 16 by shifts, then across rows by broadcasts of a row's last
+// lane (six additions with a data-parallel operand; shuffles through the LDS unit take ten times as long, and a
+// small product waits for this before it can load anything).
+FX_DEV int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // row_bcast:31 into rows 2 and 3
     return v;
 }
+FX_DEV int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // Expert e0 + lane of a step over 64 experts: its first row and its rows (cut to what is left), given the rows before
 // the step; moves row_base behind the step.
 FX_DEV void group_rows(const int32_t* COUNTS, int E, int e0, int total_rows, int lane, int& row_base, int& row0, int& rows) {
     const int c = e0 + lane < E ? min(max(COUNTS[e0 + lane], 0), total_rows) : 0;
-    const int sum = wave_scan(c, lane);
+    const int sum = wave_scan(c);
     row0 = min(row_base + sum - c, total_rows);
     rows = min(c, total_rows - row0);
-    row_base = min(row_base + uniform(__shfl(sum, 63, 64)), total_rows);
+    row_base = min(row_base + lane_value(sum, 63), total_rows);
 }
 
 struct GroupTile {     // (the same in every lane, and held in scalar registers)
@@ -121,18 +212,18 @@ FX_DEV GroupTile find_group_tile(const int32_t* COUNTS, int E, int tile, int64_t
         int row0, rows;
         group_rows(COUNTS, E, e0, (int)total_rows, lane, row_base, row0, rows);
         const int nt = (rows + (1 << SHIFT) - 1) >> SHIFT;
-        const int it = tile_base + wave_scan(nt, lane);
+        const int it = tile_base + wave_scan(nt);
         const unsigned long long who = __ballot(tile >= it - nt && tile < it);
         if (who != 0ull) {
-            const int src = (int)__builtin_ctzll(who);
+            const int src = uniform((int)__builtin_ctzll(who));
             GroupTile t;
-            t.e = uniform(e0 + src);
-            t.row0 = uniform(__shfl(row0, src, 64));
-            t.rows = uniform(__shfl(rows, src, 64));
-            t.m0 = uniform((tile - __shfl(it - nt, src, 64)) << SHIFT);
+            t.e = e0 + src;
+            t.row0 = lane_value(row0, src);
+            t.rows = lane_value(rows, src);
+            t.m0 = (tile - lane_value(it - nt, src)) << SHIFT;
             return t;
         }
-        tile_base = uniform(__shfl(it, 63, 64));
+        tile_base = lane_value(it, 63);
     }
     return GroupTile{-1, 0, 0, 0};
 }
@@ -146,9 +237,7 @@ FX_DEV int count_group_tiles(const int32_t* COUNTS, int E, int64_t total_rows, i
         group_rows(COUNTS, E, e0, (int)total_rows, lane, row_base, row0, rows);
         n += (rows + (1 << SHIFT) - 1) >> SHIFT;
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-    return uniform(n);
+    return lane_value(wave_scan(n), 63);
 }
 
 // Rows of expert e, and where they start when every expert's rows begin at a multiple of 128.
@@ -161,11 +250,9 @@ FX_DEV GroupSpan find_group_span(const int32_t* COUNTS, int E, int e, int64_t ca
     for (int e0 = 0; e0 <= e; e0 += 64) {
         const int i = e0 + lane;
         const int c = i < E ? min(max(COUNTS[i], 0), (int)capacity) : 0;
-        int p = i < e ? (c + 127) & ~127 : 0;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) p += __shfl_xor(p, off, 64);
-        padded0 = min(padded0 + uniform(p), (int)capacity);
-        if (e < e0 + 64) mine = uniform(__shfl(c, e - e0, 64));
+        const int p = i < e ? (c + 127) & ~127 : 0;
+        padded0 = min(padded0 + lane_value(wave_scan(p), 63), (int)capacity);
+        if (e < e0 + 64) mine = lane_value(c, e - e0);
     }
     GroupSpan s;
     s.padded0 = padded0;

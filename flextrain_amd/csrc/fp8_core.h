@@ -8,6 +8,8 @@
 // 64 cycles, twice as long as the 16-bit one on the same number of bytes, so a K-step costs the matrix pipe and the
 // LDS exactly what a 64-wide K-step of the 16-bit core costs them, for twice the arithmetic.
 #pragma once
+#include <math.h>
+
 #include "fp8.h"
 #include "gemm_core2.h"
 
@@ -374,6 +376,8 @@ struct Fp8Loop {
 // 256-byte runs per store) cost 33,000 cycles per 256 x 256 tile, half the K loop of a 2048-long contraction.
 // LAND: before the first store, everything this wave has requested so far must have landed (loads and stores share one
 // counter: a wait placed after the stores would also wait for them to drain).
+// (Non-temporal C reads and D stores: expert weight gradients 593 -> 678 us; a row's 128 bytes leave in four pieces that
+// the L2 has to put together.)
 template <typename TD, int TM, int TN, bool LAND>
 FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc, TD* D, int64_t ldd, int row_base, int col_base,
                          int M, int N, int lane) {
@@ -470,7 +474,7 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
 
 // ---------------------------------------------------------------- kernels over a list of tiles
 // A Source names the tiles of a launch: total(lane) how many there are, locate(id, lane) where tile `id` lies (a small
-// struct), job(where) its operands.  Counts of experts are read by whole waves (find_group_tile), so every lane calls.
+// struct), locate_one(id, lane, where) the same without the total (false: no such tile), job(where) its operands.  Counts of experts are read by whole waves (find_group_tile), so every lane calls.
 
 // 256 x 256 tiles, eight waves of 128 x 64, one workgroup per CU that walks the list with the grid as stride (Fp8Loop::run
 // keeps its loads going over the tile boundaries).  LDS: two stages of 64 KB.
@@ -571,9 +575,9 @@ template <int AF, typename TD, int MT, int NT, int NW, int U, typename Source>
 __global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
     __shared__ f32x4v_t red[NW][MT * NT][64];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const int total = src.total(lane);
-    if ((int)blockIdx.x >= total) return;
-    const Fp8Job<TD> j = src.job(src.locate(blockIdx.x, total, lane));
+    typename Source::Where where;
+    if (!src.locate_one(blockIdx.x, lane, where)) return;
+    const Fp8Job<TD> j = src.job(where);
     const int r = lane & 15, h = lane >> 4;
     const uint8_t *pa[MT], *pb[NT], *sa[MT], *sb[NT];
 #pragma unroll
@@ -678,6 +682,32 @@ __global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
         }
     }
 }
+
+// ---------------------------------------------------------------- which kernel
+// Times in microseconds, fitted to sweeps of M in 1 .. 2048, N and K in 1000 .. 14336 (dense) and of 8 .. 65536 rows over
+// 128 experts (within 15 % of what was measured except where the weights' bytes bind every form alike):
+//   small   4 + max(1, workgroups / 256) * steps * (MT + NT) * 0.05      a CU takes in 40 KB of operands per us
+//   128     4 + steps * 0.62 up to one workgroup per CU, 0.95 at two, then 1.1 for every further 512
+//   256     4 + rounds of 256 * (steps * 1.5 + 5)
+// steps: 128-long K-steps.  Examples (measured): 64 x 4096 x 4096 small 2 x 2 10.2, 128 15.4; 512 x 4096 x 4096 small 32.9,
+// 128 23.9, 256 41.5; 1024 x 14336 x 4096 128 76.6, 256 59.4.
+struct Fp8Small { int mt, nt; };
+constexpr Fp8Small kFp8Small[] = {{1, 1}, {1, 2}, {1, 4}, {2, 2}, {2, 4}, {4, 2}, {4, 4}};
+constexpr int kFp8Smalls = sizeof(kFp8Small) / sizeof(kFp8Small[0]);
+
+static inline double fp8_time_small(const Fp8Small& c, double tiles_m, int N, int steps) {
+    const double w = tiles_m * (double)((N + 16 * c.nt - 1) / (16 * c.nt)) / 256.0;
+    return 4.0 + (w > 1.0 ? w : 1.0) * steps * (c.mt + c.nt) * 0.05;
+}
+static inline double fp8_time_128(double workgroups, double steps) {
+    if (workgroups <= 256.0) return 4.0 + steps * 0.62;
+    if (workgroups <= 512.0) return 4.0 + steps * (0.62 + 0.33 * (workgroups / 256.0 - 1.0));
+    return 4.0 + ceil(workgroups / 512.0) * steps * 1.1;
+}
+static inline double fp8_time_256(double tiles, double steps) { return 4.0 + ceil(tiles / 256.0) * (steps * 1.5 + 5.0); }
+
+// Waves and K-steps in flight of the small kernel: the four forms that were fastest for their tile.
+template <int MT, int NT> struct Fp8SmallShape { static constexpr int NW = (MT == 2 || NT * MT == 16) ? 4 : 8, U = MT * NT == 1 ? 4 : MT == 4 ? 1 : 2; };
 
 static inline int fp8_cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

@@ -28,6 +28,10 @@ struct Fp8Dense {
         tile_coords(id, tiles_m, tiles_n, tm, tn);
         return Where{tm * BM, tn * BN};
     }
+    FX_DEV bool locate_one(int id, int, Where& w) const {
+        w = Where{(id / tiles_n) * BM, (id % tiles_n) * BN};
+        return true;
+    }
     FX_DEV Fp8Job<TD> job(const Where& w) const { return Fp8Job<TD>{A, B, w.m0, w.n0, K, nullptr, 0, C, D}; }
 };
 
@@ -70,29 +74,53 @@ __global__ __launch_bounds__(256) void fp8_split_reduce_kernel(const float* __re
     }
 }
 
-struct Fp8Plan { int tile, splits, k_slice; };      // tile 256 or 128; 16, 32, 64: the small kernel with that many rows
+struct Fp8Plan { int tile, small, splits, k_slice; };      // tile 256, 128, or 0: the small kernel's form `small`
 
-// 256 x 256 tiles (one workgroup per CU) when there are enough of them to fill the GPU; else 128 x 128, with the
-// contraction cut into slices of at least 4 K-steps while the workgroups still do not fill it.
+// The fastest form by the times of fp8_core.h; 128-row tiles may cut the contraction into slices (blockIdx over tile and
+// slice), which costs a second launch and 4 bytes an element and slice through memory.
 static Fp8Plan fp8_plan(int M, int N, int K) {
-    if (M <= 16) return Fp8Plan{16, 1, K};
-    if (M <= 32) return Fp8Plan{32, 1, K};
-    if (M <= 64 || K < FP8_BK) return Fp8Plan{64, 1, K};       // (the tile loads want a whole block)
-    const int64_t big = (int64_t)fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
-    if (big >= 192) return Fp8Plan{256, 1, K};
-    const int64_t small = (int64_t)fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
     const int steps = fp8_cdiv(K, FP8_BK);
-    int splits = 1;
-    if (small < 256 && steps >= 8) {
-        splits = (int)(512 / small);
-        if (splits > steps / 4) splits = steps / 4;
-        if (splits > 16) splits = 16;
-        if (splits < 1) splits = 1;
+    Fp8Plan best{0, 0, 1, K};
+    double t_best = 1e30;
+    for (int i = 0; i < kFp8Smalls; ++i) {
+        const Fp8Small& c = kFp8Small[i];
+        if (c.mt > 1 && 16 * c.mt >= 2 * M) continue;               // at least half of it would be padding
+        const double t = fp8_time_small(c, (double)fp8_cdiv(M, 16 * c.mt), N, steps);
+        if (t < t_best) { t_best = t; best = Fp8Plan{0, i, 1, K}; }
     }
-    const int slice = fp8_cdiv(steps, splits) * FP8_BK;
-    splits = fp8_cdiv(K, slice);
-    if (splits > 1 && K - (splits - 1) * slice < FP8_BK) --splits;      // the last slice takes what is short of a block
-    return Fp8Plan{128, splits, slice};
+    if (K < FP8_BK) return best;                                    // (the tile loads want a whole block)
+    const double tiles = (double)fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
+    for (int want = 1; want <= 16; want *= 2) {
+        const int slice = fp8_cdiv(steps, want) * FP8_BK;
+        int splits = fp8_cdiv(K, slice);
+        if (splits > 1 && K - (splits - 1) * slice < FP8_BK) --splits;      // the last slice takes what is short of a block
+        if (splits != want && want > 1) break;
+        if (want > 1 && (steps / want < 4 || tiles * splits > 512.0)) break;
+        double t = fp8_time_128(tiles * splits, (double)(slice / FP8_BK));
+        if (splits > 1) t += 5.0 + (double)M * N * 4.0 * (2 * splits + 1) / 4.0e6;
+        if (t < t_best) { t_best = t; best = Fp8Plan{128, 0, splits, splits > 1 ? slice : K}; }
+    }
+    if (fp8_time_256((double)fp8_cdiv(M, 256) * fp8_cdiv(N, 256), steps) < t_best) best = Fp8Plan{256, 0, 1, K};
+    return best;
+}
+
+template <int AF, typename TD, int MT, int NT>
+static void launch_small(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
+    typedef Fp8Dense<TD, 16 * MT, 16 * NT> Source;
+    typedef Fp8SmallShape<MT, NT> Shape;
+    const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(a.ext, 16 * MT), fp8_cdiv(b.ext, 16 * NT)};
+    fp8_small_kernel<AF, TD, MT, NT, Shape::NW, Shape::U, Source><<<dim3((unsigned)(src.tiles_m * src.tiles_n)), Shape::NW * 64, 0, stream>>>(src);
+}
+
+template <int AF, typename TD>
+static void launch_walk(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
+    typedef Fp8Dense<TD, 256, 256> Source;
+    const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(a.ext, 256), fp8_cdiv(b.ext, 256)};
+    const int64_t total = (int64_t)src.tiles_m * src.tiles_n;
+    const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
+    auto kern = fp8_walk_kernel<AF, TD, Source>;
+    FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+    kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
 }
 
 template <int AF, typename TD>
@@ -100,27 +128,23 @@ static int launch_dense(const Fp8View& a, const Fp8View& b, const TD* C, int64_t
                         const Fp8Plan& p, hipStream_t stream) {
     const int M = a.ext, N = b.ext;
     if (p.tile == 256) {
-        const Fp8Dense<TD, 256, 256> src{a, b, C, D, ldc, ldd, K, fp8_cdiv(M, 256), fp8_cdiv(N, 256)};
-        const int64_t total = (int64_t)src.tiles_m * src.tiles_n;
-        const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, Fp8Dense<TD, 256, 256>>;
-        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
-        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+        launch_walk<AF, TD>(a, b, C, ldc, D, ldd, K, stream);
         FX_CHECK_LAUNCH("fx_fp8_gemm");
         return 0;
     }
-#define FX_SMALL(MT, NT, NW, U)                                                                              \
-    if (p.tile == 16 * MT) {                                                                                  \
-        typedef Fp8Dense<TD, 16 * MT, 16 * NT> Source;                                                        \
-        const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(M, 16 * MT), fp8_cdiv(N, 16 * NT)};                \
-        fp8_small_kernel<AF, TD, MT, NT, NW, U, Source><<<dim3((unsigned)(src.tiles_m * src.tiles_n)), NW * 64, 0, stream>>>(src); \
-        FX_CHECK_LAUNCH("fx_fp8_gemm");                                                                       \
-        return 0;                                                                                             \
+    if (p.tile == 0) {
+        switch (p.small) {
+            case 0: launch_small<AF, TD, 1, 1>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 1: launch_small<AF, TD, 1, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 2: launch_small<AF, TD, 1, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 3: launch_small<AF, TD, 2, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 4: launch_small<AF, TD, 2, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 5: launch_small<AF, TD, 4, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            default: launch_small<AF, TD, 4, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+        }
+        FX_CHECK_LAUNCH("fx_fp8_gemm");
+        return 0;
     }
-    FX_SMALL(1, 1, 8, 4)
-    FX_SMALL(2, 2, 8, 2)
-    FX_SMALL(4, 2, 4, 2)
-#undef FX_SMALL
     const int tiles_m = fp8_cdiv(M, 128), tiles_n = fp8_cdiv(N, 128);
     if (p.splits <= 1) {
         const Fp8Dense<TD, 128, 128> src{a, b, C, D, ldc, ldd, K, tiles_m, tiles_n};
@@ -149,7 +173,7 @@ using namespace fx;
 extern "C" size_t fx_fp8_gemm_ws_bytes(int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     const Fp8Plan p = fp8_plan(M, N, K);
-    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0;
+    return p.tile == 128 && p.splits > 1 ? sizeof(float) * (size_t)p.splits * (size_t)M * (size_t)N : 0;
 }
 
 extern "C" int fx_fp8_gemm(const void* A, int64_t lda, int a_dt, const void* SA, int64_t sa_row, int64_t sa_k, int a_tiles,
@@ -167,7 +191,7 @@ extern "C" int fx_fp8_gemm(const void* A, int64_t lda, int a_dt, const void* SA,
     const int kb = fp8_cdiv(K, FP8_BK);
     if (!fp8_scales_fit(a_tiles ? fp8_cdiv(M, 128) : M, sa_row, kb, sa_k) || !fp8_scales_fit(b_tiles ? fp8_cdiv(N, 128) : N, sb_row, kb, sb_k))
         FX_FAIL("fx_fp8_gemm: a scale tensor must span less than 2 GB, with no negative stride");
-    if ((int64_t)fp8_cdiv(M, 128) * fp8_cdiv(N, 128) > (1 << 26)) FX_FAIL("fx_fp8_gemm: too many tiles");
+    if ((int64_t)fp8_cdiv(M, 16) * fp8_cdiv(N, 16) > 0x7fffffff) FX_FAIL("fx_fp8_gemm: too many tiles");
     if (ws_bytes < fx_fp8_gemm_ws_bytes(M, N, K) || (ws && !aligned16(ws)) || (!ws && fx_fp8_gemm_ws_bytes(M, N, K) > 0))
         FX_FAIL("fx_fp8_gemm: workspace missing, misaligned or too small");
     const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, a_tiles ? 7 : 0, M};

@@ -27,6 +27,11 @@ struct Fp8GroupedRows {
         const GroupTile t = find_group_tile<SHIFT>(COUNTS, E, p / tiles_n, total_rows, lane);
         return Where{t.row0, t.e, t.rows, t.m0, (p % tiles_n) * BN};
     }
+    FX_DEV bool locate_one(int id, int lane, Where& w) const {
+        const GroupTile t = find_group_tile<SHIFT>(COUNTS, E, id / tiles_n, total_rows, lane);
+        w = Where{t.row0, t.e, t.rows, t.m0, (id % tiles_n) * BN};
+        return t.e >= 0;
+    }
     FX_DEV Fp8Job<TD> job(const Where& w) const {
         Fp8Job<TD> j{A, B, w.m0, w.n0, K, nullptr, src_rows, nullptr, D + (int64_t)w.row0 * ldd};
         j.A.ext = w.rows;
@@ -69,46 +74,95 @@ struct Fp8GroupedWgrad {
     }
 };
 
-// Tile rows (their logarithm): 256 when experts average 384 rows or more, 128 (two workgroups per CU), and the small
-// kernel's 64, 32 or 16 when they average fewer than that.
-static int fp8_rows_shift(int64_t total_rows, int E, int K) {
-    if (K < FP8_BK) return 6;                    // (the tile loads want a whole block)
-    const int64_t avg = total_rows / E;
-    return avg >= 384 ? 8 : avg >= 64 ? 7 : avg >= 32 ? 6 : avg >= 16 ? 5 : 4;
+struct Fp8RowsPlan { int shift, small; };      // tile rows (their logarithm): 8, 7, or 4 .. 6 with the small kernel's form `small`
+
+// The fastest form by the times of fp8_core.h for rows split evenly over the experts that have any, half a tile of
+// padding each.  (Measured on 128 experts, N 1536, K 2048, routed counts: 8 rows an expert small 1 x 4 73 us, 128 81;
+// 16 rows 94, 82; 64 rows 128 92, 256 100; 128 rows 125, 116; 512 rows 310, 269.)
+static Fp8RowsPlan fp8_rows_plan(int64_t rows, int E, int N, int K) {
+    const double live = (double)(E < rows ? E : rows), avg = (double)rows / live;
+    const int steps = fp8_cdiv(K, FP8_BK);
+    auto tiles = [&](int bm) { const double t = avg / bm + 0.5; return live * (avg <= 1.0 || t < 1.0 ? 1.0 : t); };
+    Fp8RowsPlan best{4, 0};
+    double t_best = 1e30;
+    for (int i = 0; i < kFp8Smalls; ++i) {
+        const Fp8Small& c = kFp8Small[i];
+        if (c.mt > 1 && 16 * c.mt >= 2 * avg) continue;
+        const double t = fp8_time_small(c, tiles(16 * c.mt), N, steps);
+        if (t < t_best) { t_best = t; best = Fp8RowsPlan{c.mt == 1 ? 4 : c.mt == 2 ? 5 : 6, i}; }
+    }
+    if (K < FP8_BK) return best;                    // (the tile loads want a whole block)
+    const double t128 = fp8_time_128(tiles(128) * fp8_cdiv(N, 128), steps);
+    if (t128 < t_best) { t_best = t128; best = Fp8RowsPlan{7, 0}; }
+    if (fp8_time_256(tiles(256) * fp8_cdiv(N, 256), steps) < t_best) best = Fp8RowsPlan{8, 0};
+    return best;
+}
+
+template <typename TD>
+struct Fp8RowsArgs {
+    Fp8View a, b;
+    int64_t b_expert, sb_expert;
+    const int32_t *counts, *map;
+    int a_rows;
+    TD* D;
+    int64_t ldd, rows;
+    int E, K;
+    template <typename Source> Source source(int tiles_n) const {
+        return Source{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, rows, E, a_rows, K, tiles_n};
+    }
+    // at most this many row tiles, whatever the split over the experts
+    int64_t most(int shift) const { return (rows >> shift) + (E < rows ? E : rows); }
+};
+
+template <int AF, typename TD, int MT, int NT>
+static int launch_rows_small(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
+    constexpr int SHIFT = MT == 1 ? 4 : MT == 2 ? 5 : 6;
+    typedef Fp8GroupedRows<TD, SHIFT, 16 * NT> Source;
+    typedef Fp8SmallShape<MT, NT> Shape;
+    const int tiles_n = fp8_cdiv(g.b.ext, 16 * NT);
+    if (g.most(SHIFT) * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
+    fp8_small_kernel<AF, TD, MT, NT, Shape::NW, Shape::U, Source><<<dim3((unsigned)(g.most(SHIFT) * tiles_n)), Shape::NW * 64, 0, stream>>>(g.template source<Source>(tiles_n));
+    return 0;
 }
 
 template <int AF, typename TD>
-static int launch_rows(const Fp8View& a, const Fp8View& b, int64_t b_expert, int64_t sb_expert, const int32_t* counts,
-                       const int32_t* map, int64_t a_rows, TD* D, int64_t ldd, int64_t total_rows, int E, int K, hipStream_t stream) {
-    const int N = b.ext;
-    const int shift = fp8_rows_shift(total_rows, E, K);
-    // at most this many row tiles, whatever the split over the experts
-    const int64_t most = (total_rows >> shift) + (E < total_rows ? E : total_rows);
-    const int tiles_n = fp8_cdiv(N, shift >= 7 ? 1 << shift : shift == 4 ? 16 : 32);
-    if (most * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
-    if (shift == 8) {
-        typedef Fp8GroupedRows<TD, 8, 256> Source;
-        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};
-        const unsigned grid = (unsigned)(most * tiles_n < fp8_walk_grid() ? most * tiles_n : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, Source>;
-        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
-        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
-#define FX_SMALL(SHIFT, MT, NT, NW, U)                                                                       \
-    } else if (shift == SHIFT) {                                                                              \
-        typedef Fp8GroupedRows<TD, SHIFT, 16 * NT> Source;                                                    \
-        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n}; \
-        fp8_small_kernel<AF, TD, MT, NT, NW, U, Source><<<dim3((unsigned)(most * tiles_n)), NW * 64, 0, stream>>>(src);
-    FX_SMALL(4, 1, 1, 8, 4)
-    FX_SMALL(5, 2, 2, 8, 2)
-    FX_SMALL(6, 4, 2, 4, 2)
-#undef FX_SMALL
-    } else {
+static int launch_rows_walk(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
+    typedef Fp8GroupedRows<TD, 8, 256> Source;
+    const int tiles_n = fp8_cdiv(g.b.ext, 256);
+    const int64_t total = g.most(8) * tiles_n;
+    if (total > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
+    const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
+    auto kern = fp8_walk_kernel<AF, TD, Source>;
+    FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+    kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(g.template source<Source>(tiles_n));
+    return 0;
+}
+
+template <int AF, typename TD>
+static int launch_rows(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
+    const Fp8RowsPlan p = fp8_rows_plan(g.rows, g.E, g.b.ext, g.K);
+    int rc = 0;
+    if (p.shift == 8) {
+        rc = launch_rows_walk<AF, TD>(g, stream);
+    } else if (p.shift == 7) {
         typedef Fp8GroupedRows<TD, 7, 128> Source;
-        const Source src{a, b, b_expert, sb_expert, counts, map, D, 0, ldd, total_rows, E, (int)a_rows, K, tiles_n};
+        const int tiles_n = fp8_cdiv(g.b.ext, 128);
+        if (g.most(7) * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
         auto kern = fp8_tile_kernel128<AF, TD, Source>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8Tile128Lds);
-        kern<<<dim3((unsigned)(most * tiles_n)), 256, kFp8Tile128Lds, stream>>>(src);
+        kern<<<dim3((unsigned)(g.most(7) * tiles_n)), 256, kFp8Tile128Lds, stream>>>(g.template source<Source>(tiles_n));
+    } else {
+        switch (p.small) {
+            case 0: rc = launch_rows_small<AF, TD, 1, 1>(g, stream); break;
+            case 1: rc = launch_rows_small<AF, TD, 1, 2>(g, stream); break;
+            case 2: rc = launch_rows_small<AF, TD, 1, 4>(g, stream); break;
+            case 3: rc = launch_rows_small<AF, TD, 2, 2>(g, stream); break;
+            case 4: rc = launch_rows_small<AF, TD, 2, 4>(g, stream); break;
+            case 5: rc = launch_rows_small<AF, TD, 4, 2>(g, stream); break;
+            default: rc = launch_rows_small<AF, TD, 4, 4>(g, stream); break;
+        }
     }
+    if (rc != 0) return rc;
     FX_CHECK_LAUNCH("fx_fp8_grouped_gemm");
     return 0;
 }
@@ -164,7 +218,7 @@ extern "C" int fx_fp8_grouped_gemm(const void* A, int64_t lda, int a_dt, const v
     const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, 0, 0};
     const Fp8View b{(const uint8_t*)B, (const uint8_t*)SB, (int)ldb, (int)sb_row, (int)sb_k, b_tiles ? 7 : 0, N};
     int rc = -1;
-    FX_DISPATCH_FP8(a_dt, AF, FX_DISPATCH_DTYPE(d_dt, TD, rc = launch_rows<AF, TD>(a, b, b_expert, sb_expert, counts, row_map, a_rows, (TD*)D, ldd, total_rows, E, K, stream)));
+    FX_DISPATCH_FP8(a_dt, AF, FX_DISPATCH_DTYPE(d_dt, TD, rc = launch_rows<AF, TD>(Fp8RowsArgs<TD>{a, b, b_expert, sb_expert, counts, row_map, (int)a_rows, (TD*)D, ldd, total_rows, E, K}, stream)));
     return rc;
 }
 

@@ -18,6 +18,43 @@ struct QuantBatch {
     int64_t x, q, s, qt, st;
 };
 
+// A lane's 8 consecutive values of a row: maximum magnitude (as fp32 bits, finite values only), and the 8 bytes they become.
+template <typename T, int FMT>
+struct Lane8 {            // 4-byte types
+    float x[8];
+    template <bool VEC> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load8_or_zero<T, VEC>(row, col, cols, x); }
+    FX_DEV unsigned mag() const {
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, finite_mag(x[j]));
+        return m;
+    }
+    // largest of a 16-lane row, as fp32 bits
+    FX_DEV unsigned block_mag() const { return row16_umax(mag()); }
+    FX_DEV uint2 bytes(int b) const {
+        const float inv = inverse_scale(b);
+        return make_uint2(pack_fp8x4<FMT>(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                          pack_fp8x4<FMT>(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv));
+    }
+};
+template <typename T, int FMT>
+struct Lane8Pairs {       // 2-byte types
+    unsigned x[4];
+    template <bool VEC> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load4_pairs<T, VEC>(row, col, cols, x); }
+    FX_DEV unsigned block_mag() const {
+        unsigned m = pk_umax(pk_umax(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu), pk_umax(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
+        m = max(m & 0xffffu, m >> 16);
+        if (__any(m >= Half<T>::INF)) {
+            m = pk_umax(pk_umax(pk_finite<T>(x[0]), pk_finite<T>(x[1])), pk_umax(pk_finite<T>(x[2]), pk_finite<T>(x[3])));
+            m = max(m & 0xffffu, m >> 16);
+        }
+        return Half<T>::f32_bits(row16_umax(m));
+    }
+    FX_DEV uint2 bytes(int b) const { return make_uint2(cvt_pairs<T, FMT>(x[0], x[1], b), cvt_pairs<T, FMT>(x[2], x[3], b)); }
+};
+template <typename T, int FMT> struct LaneOf { typedef Lane8Pairs<T, FMT> type; };
+template <int FMT> struct LaneOf<float, FMT> { typedef Lane8<float, FMT> type; };
+
 // Rows form.  A workgroup takes 16 rows x 512 columns: a wave 4 rows, one after the other, its 64 lanes
 // covering 4 blocks of 128 columns (1 KB of bf16 per load instruction).  A 16-lane group ends with the scale
 // bytes of 4 consecutive rows, which leave as one 4-byte store.
@@ -31,27 +68,18 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ X, 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t tr = blockIdx.x / tiles_c, tc = blockIdx.x % tiles_c;
     const int64_t row0 = tr * 16 + wave * 4, col = tc * 512 + lane * 8;
-    float x[4][8];
+    typename LaneOf<T, FMT>::type x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const int64_t r = row0 + u;
-        load8_or_zero<T, VEC>(X + (r < rows ? r : 0) * ldx, col, r < rows ? cols : 0, x[u]);
+        x[u].template load<VEC>(X + (r < rows ? r : 0) * ldx, col, r < rows ? cols : 0);
     }
     unsigned bytes = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        unsigned m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, finite_mag(x[u][j]));
-        const int b = scale_byte<FMT>(group_umax<16>(m));
+        const int b = scale_byte<FMT>(x[u].block_mag());
         bytes |= (unsigned)b << (8 * u);
-        const float inv = inverse_scale(b);
-        if (row0 + u < rows && col < ldq) {
-            uint2 o;
-            o.x = pack_fp8x4<FMT>(x[u][0] * inv, x[u][1] * inv, x[u][2] * inv, x[u][3] * inv);
-            o.y = pack_fp8x4<FMT>(x[u][4] * inv, x[u][5] * inv, x[u][6] * inv, x[u][7] * inv);
-            *reinterpret_cast<uint2*>(Q + (row0 + u) * ldq + col) = o;
-        }
+        if (row0 + u < rows && col < ldq) *reinterpret_cast<uint2*>(Q + (row0 + u) * ldq + col) = x[u].bytes(b);
     }
     if ((lane & 15) == 0 && col < cols) {
         uint8_t* s = S + (col >> 7) * lds + row0;
@@ -73,7 +101,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ X, 
 // ROWS / COLS: which outputs are written; TILE: one scale for all 128 x 128 values.
 // GROUPED: the row axis is the expert-padded order (find_group_tile), optionally gathered through MAP.
 template <typename T, int FMT, bool VEC, bool ROWS, bool COLS, bool TILE, bool GROUPED>
-__global__ __launch_bounds__(256) void fp8_tile_kernel(
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 6 : 3) void fp8_tile_kernel(
     const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, int64_t ldq, uint8_t* __restrict__ S, int64_t lds,
     uint8_t* __restrict__ QT, int64_t ldt, uint8_t* __restrict__ ST, int64_t ldst, int64_t rows, int64_t cols,
     unsigned tiles_c, const int32_t* __restrict__ COUNTS, int E, const int32_t* __restrict__ MAP, int64_t src_rows,
@@ -83,7 +111,7 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
     if (COLS) { QT += blockIdx.y * batch.qt; ST += blockIdx.y * batch.st; }
     constexpr int PITCH = 136;
     __shared__ __align__(16) uint8_t stage[COLS ? 128 * PITCH : 16];
-    __shared__ unsigned colmax[4][128];
+    __shared__ unsigned colmax[4][sizeof(T) == 2 ? 64 : 128];
     __shared__ unsigned tilemax[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int g = tid >> 4, c = tid & 15;
@@ -97,7 +125,9 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
         live = max(0, min(128, t.rows - t.m0));
     }
     const int64_t col = tc * 128 + c * 8;
-    float x[8][8];
+    typedef typename LaneOf<T, FMT>::type Lane;
+    constexpr bool PAIRS = sizeof(T) == 2;
+    Lane x[8];
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = g * 8 + p;
@@ -105,25 +135,14 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
         int64_t src = ok ? first + r : 0;
         // a map entry outside the source must not turn into an address outside it
         if (GROUPED && MAP != nullptr && ok) src = min(max((int64_t)MAP[src], (int64_t)0), src_rows - 1);
-        load8_or_zero<T, VEC>(X + src * ldx, col, ok ? cols : 0, x[p]);
+        x[p].template load<VEC>(X + src * ldx, col, ok ? cols : 0);
     }
-    unsigned rmax[8], cmax[8];
-#pragma unroll
-    for (int p = 0; p < 8; ++p) rmax[p] = cmax[p] = 0;
-#pragma unroll
-    for (int p = 0; p < 8; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned m = finite_mag(x[p][j]);
-            rmax[p] = max(rmax[p], m);
-            cmax[j] = max(cmax[j], m);
-        }
     int tile_b = 0;
     if (TILE) {
         unsigned m = 0;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) m = max(m, rmax[p]);
-        m = group_umax<64>(m);
+        for (int p = 0; p < 8; ++p) m = max(m, x[p].block_mag());
+        m = rows4_umax(m);
         if (lane == 0) tilemax[wave] = m;
         __syncthreads();
         tile_b = scale_byte<FMT>(max(max(tilemax[0], tilemax[1]), max(tilemax[2], tilemax[3])));
@@ -133,31 +152,51 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
         }
     }
     if (COLS && !TILE) {
+        // maxima of this lane's 8 columns over its 8 rows, then over the wave's four rows of lanes
+        if constexpr (PAIRS) {
+            unsigned m[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            unsigned m = cmax[j];
-            m = max(m, (unsigned)__shfl_xor((int)m, 16, 64));
-            m = max(m, (unsigned)__shfl_xor((int)m, 32, 64));
-            cmax[j] = m;
+            for (int d = 0; d < 4; ++d) {
+                m[d] = x[0].x[d] & 0x7fff7fffu;
+#pragma unroll
+                for (int p = 1; p < 8; ++p) m[d] = pk_umax(m[d], x[p].x[d] & 0x7fff7fffu);
+            }
+            const unsigned top = pk_umax(pk_umax(m[0], m[1]), pk_umax(m[2], m[3]));
+            if (__any(max(top & 0xffffu, top >> 16) >= Half<T>::INF)) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    m[d] = 0;
+#pragma unroll
+                    for (int p = 0; p < 8; ++p) m[d] = pk_umax(m[d], pk_finite<T>(x[p].x[d]));
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const auto a = __builtin_amdgcn_permlane16_swap(m[d], m[d], false, false);
+                m[d] = pk_umax(a[0], a[1]);
+                const auto b = __builtin_amdgcn_permlane32_swap(m[d], m[d], false, false);
+                m[d] = pk_umax(b[0], b[1]);
+                if (lane < 16) colmax[wave][c * 4 + d] = m[d];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                unsigned m = 0;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) m = max(m, finite_mag(x[p].x[j]));
+                m = rows4_umax(m);
+                if (lane < 16) colmax[wave][c * 8 + j] = m;
+            }
         }
-        if (lane < 16)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) colmax[wave][c * 8 + j] = cmax[j];
         __syncthreads();
     }
     if (ROWS) {
         unsigned lo = 0, hi = 0;
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            const int b = TILE ? tile_b : scale_byte<FMT>(group_umax<16>(rmax[p]));
+            const int b = TILE ? tile_b : scale_byte<FMT>(x[p].block_mag());
             (p < 4 ? lo : hi) |= (unsigned)b << (8 * (p & 3));
-            const float inv = inverse_scale(b);
-            if (g * 8 + p < live && col < ldq) {
-                uint2 o;
-                o.x = pack_fp8x4<FMT>(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
-                o.y = pack_fp8x4<FMT>(x[p][4] * inv, x[p][5] * inv, x[p][6] * inv, x[p][7] * inv);
-                *reinterpret_cast<uint2*>(Q + (first + g * 8 + p) * ldq + col) = o;
-            }
+            if (g * 8 + p < live && col < ldq) *reinterpret_cast<uint2*>(Q + (first + g * 8 + p) * ldq + col) = x[p].bytes(b);
         }
         if (!TILE && c == 0) {
             uint8_t* s = S + tc * lds + first + g * 8;
@@ -170,19 +209,52 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(
         }
     }
     if (COLS) {
+        unsigned cm[8];          // fp32 bits of the 8 columns' maxima
+        if (!TILE) {
+            if constexpr (PAIRS) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const int k = c * 4 + d;
+                    const unsigned m = pk_umax(pk_umax(colmax[0][k], colmax[1][k]), pk_umax(colmax[2][k], colmax[3][k]));
+                    cm[2 * d] = Half<T>::f32_bits(m & 0xffffu);
+                    cm[2 * d + 1] = Half<T>::f32_bits(m >> 16);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int k = c * 8 + j;
+                    cm[j] = max(max(colmax[0][k], colmax[1][k]), max(colmax[2][k], colmax[3][k]));
+                }
+            }
+        }
+        unsigned blo = 0, bhi = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            int b = tile_b;
-            if (!TILE) {
-                const int k = c * 8 + j;
-                b = scale_byte<FMT>(max(max(colmax[0][k], colmax[1][k]), max(colmax[2][k], colmax[3][k])));
-                if (g == 0 && col + j < cols) ST[tr * ldst + col + j] = (uint8_t)b;
-            }
-            const float inv = inverse_scale(b);
+            const int b = TILE ? tile_b : scale_byte<FMT>(cm[j]);
+            (j < 4 ? blo : bhi) |= (unsigned)b << (8 * (j & 3));
             uint2 o;
-            o.x = pack_fp8x4<FMT>(x[0][j] * inv, x[1][j] * inv, x[2][j] * inv, x[3][j] * inv);
-            o.y = pack_fp8x4<FMT>(x[4][j] * inv, x[5][j] * inv, x[6][j] * inv, x[7][j] * inv);
+            if constexpr (PAIRS) {
+                // values of one column from two rows, side by side
+                constexpr unsigned sel_lo = 0x05040100u, sel_hi = 0x07060302u;
+                const unsigned sel = (j & 1) ? sel_hi : sel_lo;
+                const int d = j >> 1;
+                o.x = cvt_pairs<T, FMT>(__builtin_amdgcn_perm(x[1].x[d], x[0].x[d], sel), __builtin_amdgcn_perm(x[3].x[d], x[2].x[d], sel), b);
+                o.y = cvt_pairs<T, FMT>(__builtin_amdgcn_perm(x[5].x[d], x[4].x[d], sel), __builtin_amdgcn_perm(x[7].x[d], x[6].x[d], sel), b);
+            } else {
+                const float inv = inverse_scale(b);
+                o.x = pack_fp8x4<FMT>(x[0].x[j] * inv, x[1].x[j] * inv, x[2].x[j] * inv, x[3].x[j] * inv);
+                o.y = pack_fp8x4<FMT>(x[4].x[j] * inv, x[5].x[j] * inv, x[6].x[j] * inv, x[7].x[j] * inv);
+            }
             *reinterpret_cast<uint2*>(stage + (c * 8 + j) * PITCH + g * 8) = o;
+        }
+        if (!TILE && g == 0) {
+            uint8_t* s = ST + tr * ldst + col;
+            if (col + 8 <= cols && (reinterpret_cast<uintptr_t>(s) & 7) == 0) {
+                *reinterpret_cast<uint2*>(s) = make_uint2(blo, bhi);
+            } else {
+                for (int j = 0; j < 8; ++j)
+                    if (col + j < cols) s[j] = (uint8_t)((j < 4 ? blo : bhi) >> (8 * (j & 3)));
+            }
         }
         __syncthreads();
 #pragma unroll

@@ -42,15 +42,16 @@ def _fp8_rows(batch, rows, cols, dtype, device):
     start at multiples of 16 bytes."""
     ld = _round_up(cols, 16)
     if batch is None:
-        q = torch.empty((rows, ld), dtype=dtype, device=device)
-        return q if ld == cols else q[:, :cols]
+        if ld == cols:
+            return torch.empty((rows, cols), dtype=dtype, device=device)
+        return torch.empty((rows, ld), dtype=dtype, device=device)[:, :cols]
     return torch.empty((batch, rows, ld), dtype=dtype, device=device)[..., :cols]
 
 
 def _scale_store(batch, rows, blocks, device):
     """Uninitialised scales ``(rows, blocks)`` / ``(batch, rows, blocks)``, the block index outermost in memory."""
     if batch is None:
-        return torch.empty((blocks, rows), dtype=_E8M0, device=device).t()
+        return torch.empty_strided((rows, blocks), (1, rows), dtype=_E8M0, device=device)
     return torch.empty((batch, blocks, rows), dtype=_E8M0, device=device).transpose(1, 2)
 
 

@@ -145,7 +145,10 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     rounded on the way); ``None`` gives ``Y`` in ``X``'s dtype, equal to ``flextrain_rmsnorm_fwd(H, W)``, and no
     scales.  ``sum_out`` receives ``H`` and may be ``X`` or ``residual``."""
     op = "flextrain_add_rmsnorm_fwd"
-    T, D, _, _ = _norm_config(X, W, None)
+    shape, dtype, device = X.shape, X.dtype, X.device
+    if len(shape) != 2 or not X.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
+        _norm_config(X, W, None)            # raises
+    T, D = shape
     if D == 0:
         raise ValueError(f"{op}: X has no columns")
     if residual is not None:
@@ -153,7 +156,6 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     if sum_out is not None:
         _check_like(sum_out, X, "sum_out")
     require_same_device(X, residual, W, sum_out, op=op)
-    device, dtype = X.device, X.dtype
     x_dt = dtype_enum(dtype)
     y_dt = x_dt if output_dtype is None or output_dtype == dtype else fp8_enum(output_dtype)
     H = sum_out

@@ -264,6 +264,18 @@ inline int cvt_pk_8(float a, float b, int old, bool high, bool e5m2) {
     return high ? (int)(((unsigned)old & 0xffffu) | (two << 16)) : (int)(((unsigned)old & 0xffff0000u) | two);
 }
 
+// v_cvt_scalef32_pk_{fp8,bf8}_{bf16,f16}: a pair divided by the power of two in the scale's exponent field, rounded once
+template <typename S2, typename P2>
+inline S2 cvt_scale_pk_8(S2 old, P2 src, float scale, bool high, bool e5m2) {
+    unsigned bits;
+    memcpy(&bits, &scale, 4);
+    const int e = (int)((bits >> 23) & 255u) - 127;
+    auto one = [&](float v) { return fp8_code((float)ldexp((double)v, -e), e5m2); };     // (2-byte values: exact in fp32 unless tiny)
+    const unsigned two = one((float)src[0]) | ((unsigned)one((float)src[1]) << 8);
+    old[high ? 1 : 0] = (short)two;
+    return old;
+}
+
 // v_mfma_scale_f32_32x32x64_f8f6f4 with 8-bit operands: D = A (32 x 64) * B (64 x 32) + C, every 32 k of an
 // operand row times 2^(byte - 127) (byte 255: NaN).  Lane l supplies A[l % 32][32 (l / 32) .. + 31], B likewise,
 // and the scale bytes of those values; the accumulator layout is that of the 16-bit instruction.
@@ -297,8 +309,28 @@ inline Acc mfma_scale(Frag a, Frag b, Acc c, int fmt_a, int fmt_b, int opsel_a, 
     return c;
 }
 
-// v_permlane32_swap: the upper 32 lanes of the first operand change places with the lower 32 of the second.
+// Data-parallel operand of v_mov: row_shr:1..15 (0x111 ..), row_bcast:15 (0x142), row_bcast:31 (0x143).  A lane whose row is
+// not in row_mask, or whose source does not exist, keeps `old`.
+inline int update_dpp(int old, int v, int ctrl, int row_mask) {
+    const unsigned l = flat_thread() & 63u, row = l >> 4;
+    int src = -1;
+    if (ctrl >= 0x111 && ctrl <= 0x11f) { const unsigned n = (unsigned)ctrl - 0x110; if ((l & 15u) >= n) src = (int)(l - n); }
+    else if (ctrl >= 0x121 && ctrl <= 0x12f) src = (int)((l & ~15u) | ((l - ((unsigned)ctrl - 0x120)) & 15u));       // row_ror
+    else if (ctrl == 0x142) { if (row >= 1) src = (int)(row * 16 - 1); }
+    else if (ctrl == 0x143) { if (row >= 2) src = 31; }
+    else { fprintf(stderr, "hostsim: data-parallel control 0x%x\n", ctrl); abort(); }
+    const int got = exchange(v, src < 0 ? (int)l : src);
+    return src >= 0 && ((row_mask >> row) & 1) ? got : old;
+}
+// v_permlane16_swap: the odd rows of 16 lanes of the first operand change places with the even rows of the second.
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+inline u32x2_t permlane16_swap(unsigned a, unsigned b) {
+    const unsigned l = flat_thread() & 63u;
+    const unsigned b_even = exchange(b, (int)(l & ~16u)), a_odd = exchange(a, (int)(l | 16u));
+    u32x2_t out = {l & 16u ? b_even : a, l & 16u ? b : a_odd};
+    return out;
+}
+// v_permlane32_swap: the upper 32 lanes of the first operand change places with the lower 32 of the second.
 inline u32x2_t permlane32_swap(unsigned a, unsigned b) {
     const unsigned l = flat_thread() & 63u;
     const unsigned b_lo = exchange(b, (int)(l & 31u)), a_hi = exchange(a, (int)((l & 31u) + 32u));
@@ -335,6 +367,13 @@ inline unsigned perm_b32(unsigned hi, unsigned lo, unsigned sel) {
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) hostsim::mfma32x32x16(a, b, c)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<32>(a, b, c, fa, fb, oa, sa, ob, sb)
 #define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) hostsim::mfma_scale<16>(a, b, c, fa, fb, oa, sa, ob, sb)
+#define __builtin_amdgcn_permlane16_swap(a, b, fi, bc) hostsim::permlane16_swap(a, b)
+#define __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, src, scale, high) hostsim::cvt_scale_pk_8(old, src, scale, high, false)
+#define __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(old, src, scale, high) hostsim::cvt_scale_pk_8(old, src, scale, high, true)
+#define __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, src, scale, high) hostsim::cvt_scale_pk_8(old, src, scale, high, false)
+#define __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(old, src, scale, high) hostsim::cvt_scale_pk_8(old, src, scale, high, true)
+#define __builtin_amdgcn_update_dpp(old, v, ctrl, rows, banks, bound) hostsim::update_dpp(old, v, ctrl, rows)
+#define __builtin_amdgcn_readlane(v, lane) hostsim::exchange((int)(v), (int)(lane))
 #define __builtin_amdgcn_permlane32_swap(a, b, fi, bc) hostsim::permlane32_swap(a, b)
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, false)
 #define __builtin_amdgcn_cvt_pk_bf8_f32(a, b, old, high) hostsim::cvt_pk_8(a, b, old, high, true)

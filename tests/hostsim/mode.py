@@ -183,3 +183,10 @@ def activate():
     for name in ("empty", "zeros", "ones", "full", "tensor", "randn", "rand", "arange", "randint", "empty_like", "zeros_like",
                  "ones_like", "full_like", "randn_like", "rand_like"):
         setattr(torch, name, _host_only(getattr(torch, name), poison=name in ("empty", "empty_like")))
+
+    def empty_strided(size, stride, **kwargs):
+        """Its storage from the patched torch.empty: guarded and poisoned like any other."""
+        span = 1 + sum((n - 1) * step for n, step in zip(size, stride)) if all(size) else 0
+        return torch.empty(span, **kwargs).as_strided(size, stride)
+
+    torch.empty_strided = empty_strided

@@ -232,16 +232,53 @@ def test_matmul(dev, m, n, k, fmt, b_tiles):
     assert torch.equal(acc, out)
 
 
-@pytest.mark.parametrize("m,n,k", [(8200, 1540, 200), (2050, 6300, 384), (300, 12000, 128)])
-def test_matmul_many_tiles(dev, m, n, k):
-    """Enough tiles to fill the GPU: the launch whose workgroups walk several 256 x 256 tiles."""
+def some_rows(g, m):
+    """Row numbers to check of a large output: the first and last ones and some between."""
+    return torch.cat([torch.arange(min(m, 8)), torch.arange(max(0, m - 8), m), torch.randint(0, m, (32,), generator=g)])
+
+
+# 128 x 128 tiles; the same with the contraction in slices; 256 x 256 tiles, several to a workgroup
+@pytest.mark.parametrize("m,n,k", [(8200, 1540, 200), (2050, 6300, 384), (300, 12000, 128), (1030, 4100, 1999), (300, 310, 14010), (333, 5000, 8008),
+                                   (4200, 3700, 1200), (8300, 7900, 1100), (2100, 14336, 1024)])
+def test_matmul_large(dev, m, n, k):
     g = gen(m)
     a, sa, av = operand(dev, values(g, m, k, sigma=1e-3), E5M2)
     b, sb, bv = operand(dev, values(g, n, k, sigma=k ** -0.5), tiles=True)
+    some = some_rows(g, m)
+    av = av[some]
     ref = av @ bv.t()
     c = values(g, m, n, sigma=float(ref.std()))
-    check(ops.flextrain_fp8_matmul(a, sa, b, sb), ref, av, bv)
-    check(ops.flextrain_fp8_matmul(a, sa, b, sb, C=c.to(dev)), ref + c.double(), av, bv, c)
+    check(ops.flextrain_fp8_matmul(a, sa, b, sb)[some], ref, av, bv)
+    cd = c.to(dev)
+    out = ops.flextrain_fp8_matmul(a, sa, b, sb, C=cd)
+    check(out[some], ref + c[some].double(), av, bv, c[some])
+    assert ops.flextrain_fp8_matmul(a, sa, b, sb, C=cd, out=cd) is cd and torch.equal(cd, out)
+    for t in (torch.float16, torch.float32):
+        check(ops.flextrain_fp8_matmul(a, sa, b, sb, out_dtype=t)[some], ref, av, bv, what=str(t))
+
+
+@pytest.mark.parametrize("E,avg,n,k", [(64, 40, 1536, 1024), (64, 40, 1500, 1000), (16, 300, 1600, 1032), (16, 700, 2000, 1160), (128, 8, 1536, 512)])
+def test_grouped_matmul_large(dev, E, avg, n, k):
+    """128- and 256-row tiles, gathered and sorted, with experts of every size, some without rows."""
+    g = gen(E + n)
+    counts = torch.randint(0, 2 * avg, (E,), generator=g, dtype=torch.int32)
+    counts[3] = 0
+    rows = int(counts.sum())
+    w = (torch.randn(E, n, k, generator=g) * k ** -0.5).to(torch.bfloat16)
+    b, sb = ops.flextrain_fp8_quantize(w.to(dev), tiles=True)
+    source = torch.randint(0, 500, (rows,), generator=g, dtype=torch.int32)
+    start = torch.cumsum(counts, 0) - counts
+    for gathered in (False, True):
+        a, sa, av = operand(dev, values(g, 500 if gathered else rows, k), E5M2 if gathered else E4M3)
+        if gathered:
+            av = av[source.long()]
+        out = ops.flextrain_fp8_grouped_matmul(a, sa, b, sb, counts.to(dev), row_sources=source.to(dev) if gathered else None)
+        for e in (0, 1, 3, E // 2, E - 1):
+            at, c = int(start[e]), int(counts[e])
+            if c:
+                some = at + some_rows(g, c)
+                bv = o.dequantize(b[e].cpu(), sb[e].cpu(), 128)
+                check(out[some], av[some] @ bv.t(), av[some], bv, what=f"expert {e}")
 
 
 def test_matmul_tiles_on_both_sides_and_strides(dev):
