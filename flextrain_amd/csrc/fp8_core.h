@@ -78,7 +78,7 @@ struct Fp8Loop {
     static constexpr int STAGE = (BM + BN) * FP8_BK;                            // bytes
     static constexpr int HI = TM / 2;                                           // A fragments with two register sets
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile rows must split evenly over the waves");
-    static_assert(TM >= 2 && TM % 2 == 0 && TM <= 4 && TN == 2, "fragment schedule below");
+    static_assert((TM == 2 && TN == 2) || (TM == 4 && (TN == 2 || TN == 4)), "fragment schedule below");
     static constexpr int PER = (LD + MFMAS - 1) / MFMAS;
 
     // fragments: a sub-step (64 k) needs TM of A and TN of B.  B and the upper half of A have two register sets that
@@ -87,10 +87,10 @@ struct Fp8Loop {
     i32x8_t alo[TM - HI], ahi[2][HI], bf[2][TN];
     unsigned aoff[NA], boff[NB];          // lane byte offsets of the tile loads
     const uint8_t *abase, *bbase;
-    unsigned soa[TM / 2], sob;            // lane offsets of the scales: lane l fetches rows l, 64 + l, .. of its wave's
+    unsigned soa[TM / 2], sob[TN / 2];    // lane offsets of the scales: lane l fetches rows l, 64 + l, .. of its wave's
     const uint8_t *sabase, *sbbase;
     int sak, sbk;
-    int rawa[TM / 2], rawb;               // scale bytes requested for the next K-step
+    int rawa[TM / 2], rawb[TN / 2];       // scale bytes requested for the next K-step
     int sca, scb;                         // packed scales of the current one
     int wave, lane;
     unsigned lds_lane;
@@ -123,22 +123,28 @@ struct Fp8Loop {
             FX_OPAQUE(o);             // a 32-bit offset here, not a 64-bit one kept in a register pair
             rawa[i] = uniform_ptr(sabase)[o];
         }
-        unsigned o = sob;
-        FX_OPAQUE(o);
-        rawb = uniform_ptr(sbbase)[o];
+#pragma unroll
+        for (int i = 0; i < TN / 2; ++i) {
+            unsigned o = sob[i];
+            FX_OPAQUE(o);
+            rawb[i] = uniform_ptr(sbbase)[o];
+        }
         sabase += sak;
         sbbase += sbk;
     }
     // Byte i of the packed scales belongs to fragment i, whose row in lane l is 32 i + l % 32; lane l has fetched the
     // bytes of rows 64 u + l.  Exchanging the upper half of one copy with the lower half of another leaves the bytes of
     // rows 64 u + l % 32 in the first and those of rows 64 u + 32 + l % 32 in the second.
-    FX_DEV void pack_scales(int& a, int& b) const {
-        unsigned w = (unsigned)rawa[0];
-        if constexpr (TM == 4) w |= (unsigned)rawa[1] << 16;
+    template <int T>
+    static FX_DEV int pack(const int (&raw)[T]) {
+        unsigned w = (unsigned)raw[0];
+        if constexpr (T == 2) w |= (unsigned)raw[1] << 16;
         const auto x = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-        a = (int)(x[0] | (x[1] << 8));
-        const auto y = __builtin_amdgcn_permlane32_swap((unsigned)rawb, (unsigned)rawb, false, false);
-        b = (int)(y[0] | (y[1] << 8));
+        return (int)(x[0] | (x[1] << 8));
+    }
+    FX_DEV void pack_scales(int& a, int& b) const {
+        a = pack(rawa);
+        b = pack(rawb);
     }
 
     FX_DEV void init() {
@@ -199,7 +205,8 @@ struct Fp8Loop {
         bbase = j.B.p + (int64_t)j.n0 * j.B.ld;
 #pragma unroll
         for (int i = 0; i < TM / 2; ++i) soa[i] = (unsigned)((int)a_row(j, wm * WM + i * 64 + lane) >> j.A.s_shift) * (unsigned)j.A.s_row;
-        sob = (unsigned)(min(j.n0 + wn * WN + lane, j.B.ext - 1) >> j.B.s_shift) * (unsigned)j.B.s_row;
+#pragma unroll
+        for (int i = 0; i < TN / 2; ++i) sob[i] = (unsigned)(min(j.n0 + wn * WN + i * 64 + lane, j.B.ext - 1) >> j.B.s_shift) * (unsigned)j.B.s_row;
         sabase = j.A.s;
         sbbase = j.B.s;
         sak = j.K > FP8_BK ? j.A.s_k : 0;         // (a contraction of one block has one scale)
@@ -249,7 +256,13 @@ struct Fp8Loop {
             else acc[i][j] = mfma_fp8<AF, j, i>(bf[P][j], ahi[P][i - (TM - HI)], acc[i][j], scb, sca);
             if constexpr (FETCH) {
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (TM == 4) {
+                if constexpr (TN == 4) {
+                    if constexpr (M < 4) read_b<M % 4, Q>(buf, ks_f);
+                    if constexpr (M == 4) read_a<0, Q>(buf, ks_f);     // its last MFMA was M == 3
+                    if constexpr (M == 5) read_a<2, Q>(buf, ks_f);
+                    if constexpr (M == 6) read_a<3, Q>(buf, ks_f);
+                    if constexpr (M == 8) read_a<1, Q>(buf, ks_f);     // its last MFMA was M == 7
+                } else if constexpr (TM == 4) {
                     if constexpr (M == 0) read_b<0, Q>(buf, ks_f);
                     if constexpr (M == 1) read_b<1, Q>(buf, ks_f);
                     if constexpr (M == 2) read_a<0, Q>(buf, ks_f);     // its last MFMA was M == 1
@@ -370,105 +383,108 @@ struct Fp8Loop {
     }
 };
 
-// D (+ C) of one wave from its accumulators, straight from registers.  Lane (r, h) = (lane % 32, lane / 32) holds of row
-// 32 i + r the columns 32 j + 8 g + 4 h .. + 3 (g = 0 .. 3): swapping the upper half-wave of group 2 q with the lower one
-// of group 2 q + 1 leaves it 8 consecutive columns, 16 bytes of a 2-byte type.  Staging the tile through LDS instead (full
-// 256-byte runs per store) cost 33,000 cycles per 256 x 256 tile, half the K loop of a 2048-long contraction.
+// D (+ C) of one wave from its accumulators, a band of 32 rows at a time through 4 KB of LDS of its own (`st`), so that a
+// load or store instruction of a wave covers eight whole 128-byte pieces of rows.
+//   accumulator side  lane (r, h) = (lane % 32, lane / 32) holds of row 32 i + r the columns 32 j + 8 g + 4 h .. + 3
+//                     (g = 0 .. 3); swapping the upper half-wave of group 2 q with the lower one of group 2 q + 1 leaves
+//                     it 8 consecutive columns
+//   memory side       lane l holds 16-byte chunk l % 8 of rows l / 8, l / 8 + 8, ..
+// Chunk c of staged row r sits at c ^ ((r >> 1) & 7): 16 lanes of either side touch every bank once.  C comes in on the
+// memory side (all bands of a 2-byte type requested at once), is added in fp32 on the accumulator side, and the sum is
+// rounded once.  Straight 16-byte stores from the accumulator side (32 bytes of each of 32 rows per instruction) took
+// 593 us for the expert weight gradients, which move 1.6 GB of C and D.
 // LAND: before the first store, everything this wave has requested so far must have landed (loads and stores share one
 // counter: a wait placed after the stores would also wait for them to drain).
-// (Non-temporal C reads and D stores: expert weight gradients 593 -> 678 us; a row's 128 bytes leave in four pieces that
-// the L2 has to put together.)
+constexpr int FP8_STAGE_BYTES = 4096;      // per wave
+
 template <typename TD, int TM, int TN, bool LAND>
 FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc, TD* D, int64_t ldd, int row_base, int col_base,
-                         int M, int N, int lane) {
+                         int M, int N, uint8_t* st, int lane) {
     typedef typename VecOf<TD>::type Pack;
-    constexpr int PN = 8 / VecOf<TD>::N;                     // 16-byte packs of 8 columns
-    constexpr int CB = PN == 1 ? TM : (TM + 1) / 2;          // row bands whose C is requested together
-    const int r = lane & 31, h = lane >> 5;
-    const bool vec = (ldd % VecOf<TD>::N) == 0 && (reinterpret_cast<uintptr_t>(D) & 15u) == 0 &&
-                     (C == nullptr || ((ldc % VecOf<TD>::N) == 0 && (reinterpret_cast<uintptr_t>(C) & 15u) == 0));
-    // wave-uniform: every row and column of this wave exists
-    const bool full = vec && row_base + 32 * TM <= M && col_base + 32 * TN <= N;
-    auto gather = [&](int i, int j, int q, float (&v)[8]) {
+    static_assert(TN == 2, "a staged row holds 64 columns of a 2-byte type or 32 of a 4-byte one");
+    constexpr int CE = VecOf<TD>::N;                         // values of a 16-byte chunk
+    constexpr int JP = sizeof(TD) == 2 ? TN : 1, PASS = TN / JP;
+    constexpr int CB = sizeof(TD) == 2 ? TM : (TM + 1) / 2;  // bands whose C is requested together
+    const int r = lane & 31, h = lane >> 5, rr = lane >> 3, ch = lane & 7;
+    const bool vec = (ldd % CE) == 0 && (reinterpret_cast<uintptr_t>(D) & 15u) == 0 &&
+                     (C == nullptr || ((ldc % CE) == 0 && (reinterpret_cast<uintptr_t>(C) & 15u) == 0));
+    auto at = [&](int row, int c) { return reinterpret_cast<Pack*>(st + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
+    Pack c[CB][PASS][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float lo = acc[i][j][8 * q + e], hi = acc[i][j][8 * q + 4 + e];
-            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
-            v[e] = __builtin_bit_cast(float, (unsigned)x[0]);
-            v[4 + e] = __builtin_bit_cast(float, (unsigned)x[1]);
-        }
-    };
-    if (full && C == nullptr) {
-        if (LAND) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        TD* d0 = D + (int64_t)(row_base + r) * ldd + col_base + h * 8;
+    for (int i = 0; i < TM; ++i) {
+        if (C != nullptr && i % CB == 0) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+            for (int b = 0; b < CB; ++b)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+                for (int s = 0; s < PASS; ++s)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    float v[8];
-                    gather(i, j, q, v);
-                    store_f32<TD, 8>(d0 + (int64_t)i * 32 * ldd + j * 32 + q * 16, v);
-                }
-    } else if (full) {
-        Pack c[CB][TN][2][PN];
-        const TD* c0 = C + (int64_t)(row_base + r) * ldc + col_base + h * 8;
-        TD* d0 = D + (int64_t)(row_base + r) * ldd + col_base + h * 8;
+                    for (int t = 0; t < 4; ++t) {
+                        const int row = row_base + (i + b) * 32 + t * 8 + rr, col = col_base + s * 32 + ch * CE;
+                        if (row < M) {
+                            const TD* src = C + (int64_t)row * ldc + col;
+                            if (vec && col + CE <= N) {
+                                c[b][s][t] = *reinterpret_cast<const Pack*>(src);
+                            } else {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            if (i % CB == 0) {
-#pragma unroll
-                for (int b = 0; b < CB; ++b)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-#pragma unroll
-                            for (int u = 0; u < PN; ++u)
-                                c[b][j][q][u] = *reinterpret_cast<const Pack*>(c0 + (int64_t)(i + b) * 32 * ldc + j * 32 + q * 16 + u * VecOf<TD>::N);
-                if (LAND && i == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    float v[8];
-                    gather(i, j, q, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += (float)c[i % CB][j][q][e / VecOf<TD>::N][e % VecOf<TD>::N];
-                    store_f32<TD, 8>(d0 + (int64_t)i * 32 * ldd + j * 32 + q * 16, v);
-                }
-        }
-    } else {
-        if (LAND) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    float v[8];
-                    gather(i, j, q, v);
-                    const int row = row_base + i * 32 + r, col = col_base + j * 32 + q * 16 + h * 8;
-                    if (row >= M || col >= N) continue;
-                    TD* d = D + (int64_t)row * ldd + col;
-                    if (vec && col + 8 <= N) {
-                        if (C != nullptr) {
-                            float add[8];
-                            load_f32<TD, 8>(C + (int64_t)row * ldc + col, add);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] += add[e];
-                        }
-                        store_f32<TD, 8>(d, v);
-                    } else {
-                        for (int e = 0; e < 8 && col + e < N; ++e) {
-                            float o = v[e];
-                            if (C != nullptr) o += (float)C[(int64_t)row * ldc + col + e];
-                            d[e] = (TD)o;
+                                for (int e = 0; e < CE; ++e)
+                                    if (col + e < N) c[b][s][t][e] = src[e];
+                            }
                         }
                     }
+        }
+        if (LAND && i == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int s = 0; s < PASS; ++s) {
+            // lockstep: the previous band has been read back before this one is staged
+            if (C != nullptr) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) *at(t * 8 + rr, ch) = c[i % CB][s][t];
+            }
+            // lockstep: a wave reads back only what it wrote itself; its LDS accesses complete in order
+#pragma unroll
+            for (int jj = 0; jj < JP; ++jj)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int j = s * JP + jj;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float lo = acc[i][j][8 * q + e], hi = acc[i][j][8 * q + 4 + e];
+                        const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+                        v[e] = __builtin_bit_cast(float, (unsigned)x[0]);
+                        v[4 + e] = __builtin_bit_cast(float, (unsigned)x[1]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8 / CE; ++u) {
+                        Pack* p = at(r, jj * 4 + (q * 2 + h) * (8 / CE) + u);
+                        Pack o;
+                        if (C != nullptr) {
+                            const Pack add = *p;
+#pragma unroll
+                            for (int e = 0; e < CE; ++e) v[u * CE + e] += (float)add[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < CE; ++e) o[e] = (TD)v[u * CE + e];
+                        *p = o;
+                    }
                 }
+            // lockstep: as above
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const Pack o = *at(t * 8 + rr, ch);
+                const int row = row_base + i * 32 + t * 8 + rr, col = col_base + s * 32 + ch * CE;
+                if (row < M && col < N) {
+                    TD* d = D + (int64_t)row * ldd + col;
+                    if (vec && col + CE <= N) {
+                        *reinterpret_cast<Pack*>(d) = o;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < CE; ++e)
+                            if (col + e < N) d[e] = o[e];
+                    }
+                }
+            }
+        }
     }
 }
 
@@ -477,9 +493,9 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
 // struct), locate_one(id, lane, where) the same without the total (false: no such tile), job(where) its operands.  Counts of experts are read by whole waves (find_group_tile), so every lane calls.
 
 // 256 x 256 tiles, eight waves of 128 x 64, one workgroup per CU that walks the list with the grid as stride (Fp8Loop::run
-// keeps its loads going over the tile boundaries).  LDS: two stages of 64 KB.
+// keeps its loads going over the tile boundaries).  LDS: two stages of 64 KB, and what the epilogue stages through.
 constexpr int FP8_WALK_BM = 256, FP8_WALK_BN = 256;
-constexpr size_t kFp8WalkLds = 128 * 1024;
+constexpr size_t kFp8WalkStages = 128 * 1024, kFp8WalkLds = kFp8WalkStages + 8 * FP8_STAGE_BYTES;     // all 160 KB
 
 // A tile whose contraction is empty: C, or zeros.
 template <typename TD, int BM, int BN, int NT>
@@ -496,7 +512,7 @@ template <int AF, typename TD, typename Source>
 __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
     extern __shared__ __align__(16) unsigned char smem[];
     typedef Fp8Loop<AF, TD, FP8_WALK_BM, FP8_WALK_BN, 2, 4> Loop;
-    static_assert(2 * Loop::STAGE == (int)kFp8WalkLds, "two stages");
+    static_assert(2 * Loop::STAGE == (int)kFp8WalkStages, "two stages");
     uint8_t *buf0 = smem, *buf1 = smem + Loop::STAGE;
     Loop loop;
     loop.init();
@@ -525,22 +541,23 @@ __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
         loop.template run<true>(src.job(cur), src.job(nxt), buf0, buf1, par, acc);
         const Fp8Job<TD> j = src.job(cur);
         fp8_epilogue<TD, Loop::TM, Loop::TN, true>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 4) * Loop::WM,
-                                                   j.n0 + (loop.wave % 4) * Loop::WN, j.A.ext, j.B.ext, loop.lane);
+                                                   j.n0 + (loop.wave % 4) * Loop::WN, j.A.ext, j.B.ext,
+                                                   smem + kFp8WalkStages + loop.wave * FP8_STAGE_BYTES, loop.lane);
         if (!more) break;
         __syncthreads();          // everyone's share of the next tile's first K-steps has landed
         cur = nxt;
     }
 }
 
-// 128 x 128 tiles, four waves of 64 x 64, one tile per workgroup; 64 KB of LDS, so two workgroups share a CU and one's
+// 128 x 128 tiles, four waves of 64 x 64, one tile per workgroup; 80 KB of LDS, so two workgroups share a CU and one's
 // epilogue and first loads run under the other's K loop.
-constexpr size_t kFp8Tile128Lds = 64 * 1024;
+constexpr size_t kFp8Tile128Stages = 64 * 1024, kFp8Tile128Lds = kFp8Tile128Stages + 4 * FP8_STAGE_BYTES;
 
 template <int AF, typename TD, typename Source>
 __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
     extern __shared__ __align__(16) unsigned char smem[];
     typedef Fp8Loop<AF, TD, 128, 128, 2, 2> Loop;
-    static_assert(2 * Loop::STAGE == (int)kFp8Tile128Lds, "two stages");
+    static_assert(2 * Loop::STAGE == (int)kFp8Tile128Stages, "two stages");
     Loop loop;
     loop.init();
     const int total = src.total(loop.lane);
@@ -555,7 +572,8 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
     int par = 0;
     loop.template run<false>(j, j, smem, smem + Loop::STAGE, par, acc);
     fp8_epilogue<TD, Loop::TM, Loop::TN, false>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 2) * Loop::WM,
-                                                j.n0 + (loop.wave % 2) * Loop::WN, j.A.ext, j.B.ext, loop.lane);
+                                                j.n0 + (loop.wave % 2) * Loop::WN, j.A.ext, j.B.ext,
+                                                smem + kFp8Tile128Stages + loop.wave * FP8_STAGE_BYTES, loop.lane);
 }
 
 // Small products: one workgroup per tile of 16 MT x 16 NT, its NW waves share the contraction (wave w takes K-steps
