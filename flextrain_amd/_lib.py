@@ -46,6 +46,7 @@ _SIGNATURES = {
     "fx_rmsnorm_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float,
                                c_int, c_int, c_int, c_void_p]),
     "fx_rmsnorm_bwd_ws_bytes": (c_size_t, [c_int64, c_int]),
+    "fx_add_rmsnorm_bwd_ws_bytes": (c_size_t, [c_int64, c_int]),
     "fx_rmsnorm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                c_int, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_void_p,
                                c_size_t, c_void_p]),

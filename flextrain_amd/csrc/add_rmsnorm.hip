@@ -194,7 +194,7 @@ extern "C" int fx_add_rmsnorm_fwd(const void* x, const void* residual, const voi
     if (x_dt != DT_F32 && x_dt != DT_F16 && x_dt != DT_BF16) FX_FAIL("fx_add_rmsnorm_fwd: unsupported dtype enum %d", x_dt);
     if (w && w_dt != DT_F32 && w_dt != DT_F16 && w_dt != DT_BF16) FX_FAIL("fx_add_rmsnorm_fwd: unsupported weight dtype enum %d", w_dt);
     if (y_dt != x_dt && !is_fp8_dt(y_dt)) FX_FAIL("fx_add_rmsnorm_fwd: the output has the input's dtype or an 8-bit one");
-    if (rows > 0x7fffffff) FX_FAIL("fx_add_rmsnorm_fwd: too many rows");
+    if (rows > 0xffffff) FX_FAIL("fx_add_rmsnorm_fwd: too many rows");      // (a launch has 2^32 threads at most)
     if (rows == 0) return 0;
     if (!x || !y || !rstd || (is_fp8_dt(y_dt) && !s) || (residual && !h)) FX_FAIL("fx_add_rmsnorm_fwd: null pointer");
     if (is_fp8_dt(y_dt)) {

@@ -134,11 +134,12 @@ FX_DEV unsigned cvt_pairs(unsigned p0, unsigned p1, int byte) {
     return __builtin_bit_cast(unsigned, w);
 }
 // Eight consecutive 2-byte values of a row as four pairs, 0 behind its end.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool NT = false>
 FX_DEV void load4_pairs(const T* row, int64_t col, int64_t cols, unsigned (&o)[4]) {
     if (VEC && col < cols) {
         typedef unsigned u4_t __attribute__((ext_vector_type(4)));
-        const u4_t v = *reinterpret_cast<const u4_t*>(row + col);
+        const u4_t* p = reinterpret_cast<const u4_t*>(row + col);
+        const u4_t v = NT ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = v[d];
     } else {
@@ -259,6 +260,9 @@ FX_DEV GroupSpan find_group_span(const int32_t* COUNTS, int E, int e, int64_t ca
     s.rows = padded0 + ((mine + 127) & ~127) <= (int)capacity ? mine : 0;
     return s;
 }
+
+// A launch has fewer than 2^32 threads along an axis.
+static inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads < ((int64_t)1 << 32); }
 
 #define FX_DISPATCH_FP8(dt, FMT, ...)                                                \
     switch (dt) {                                                                    \

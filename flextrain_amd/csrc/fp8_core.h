@@ -78,7 +78,7 @@ struct Fp8Loop {
     static constexpr int STAGE = (BM + BN) * FP8_BK;                            // bytes
     static constexpr int HI = TM / 2;                                           // A fragments with two register sets
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile rows must split evenly over the waves");
-    static_assert((TM == 2 && TN == 2) || (TM == 4 && (TN == 2 || TN == 4)), "fragment schedule below");
+    static_assert((TM == 2 || TM == 4) && TN == 2, "fragment schedule below");
     static constexpr int PER = (LD + MFMAS - 1) / MFMAS;
 
     // fragments: a sub-step (64 k) needs TM of A and TN of B.  B and the upper half of A have two register sets that
@@ -256,13 +256,7 @@ struct Fp8Loop {
             else acc[i][j] = mfma_fp8<AF, j, i>(bf[P][j], ahi[P][i - (TM - HI)], acc[i][j], scb, sca);
             if constexpr (FETCH) {
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (TN == 4) {
-                    if constexpr (M < 4) read_b<M % 4, Q>(buf, ks_f);
-                    if constexpr (M == 4) read_a<0, Q>(buf, ks_f);     // its last MFMA was M == 3
-                    if constexpr (M == 5) read_a<2, Q>(buf, ks_f);
-                    if constexpr (M == 6) read_a<3, Q>(buf, ks_f);
-                    if constexpr (M == 8) read_a<1, Q>(buf, ks_f);     // its last MFMA was M == 7
-                } else if constexpr (TM == 4) {
+                if constexpr (TM == 4) {
                     if constexpr (M == 0) read_b<0, Q>(buf, ks_f);
                     if constexpr (M == 1) read_b<1, Q>(buf, ks_f);
                     if constexpr (M == 2) read_a<0, Q>(buf, ks_f);     // its last MFMA was M == 1
@@ -397,7 +391,7 @@ struct Fp8Loop {
 // counter: a wait placed after the stores would also wait for them to drain).
 constexpr int FP8_STAGE_BYTES = 4096;      // per wave
 
-template <typename TD, int TM, int TN, bool LAND>
+template <typename TD, int TM, int TN, bool LAND, bool NT>
 FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc, TD* D, int64_t ldd, int row_base, int col_base,
                          int M, int N, uint8_t* st, int lane) {
     typedef typename VecOf<TD>::type Pack;
@@ -423,7 +417,7 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
                         if (row < M) {
                             const TD* src = C + (int64_t)row * ldc + col;
                             if (vec && col + CE <= N) {
-                                c[b][s][t] = *reinterpret_cast<const Pack*>(src);
+                                c[b][s][t] = NT ? __builtin_nontemporal_load(reinterpret_cast<const Pack*>(src)) : *reinterpret_cast<const Pack*>(src);
                             } else {
 #pragma unroll
                                 for (int e = 0; e < CE; ++e)
@@ -476,7 +470,8 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
                 if (row < M && col < N) {
                     TD* d = D + (int64_t)row * ldd + col;
                     if (vec && col + CE <= N) {
-                        *reinterpret_cast<Pack*>(d) = o;
+                        if (NT) __builtin_nontemporal_store(o, reinterpret_cast<Pack*>(d));
+                        else *reinterpret_cast<Pack*>(d) = o;
                     } else {
 #pragma unroll
                         for (int e = 0; e < CE; ++e)
@@ -497,6 +492,11 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
 constexpr int FP8_WALK_BM = 256, FP8_WALK_BN = 256;
 constexpr size_t kFp8WalkStages = 128 * 1024, kFp8WalkLds = kFp8WalkStages + 8 * FP8_STAGE_BYTES;     // all 160 KB
 
+// An output larger than the cache in front of the memory goes past it (NT; C as well), so that the operands keep their place:
+// weight gradients of 128 experts, 805 MB, 558 -> 517 us.  Smaller ones stay in it for their reader and lose by passing it
+// (8192 x 8192 x 8192, 134 MB: 387 -> 402 us; 8192 x 14336 x 4096, 235 MB: 363 -> 375 us).
+constexpr size_t kFp8OnceBytes = (size_t)256 << 20;
+
 // A tile whose contraction is empty: C, or zeros.
 template <typename TD, int BM, int BN, int NT>
 FX_DEV void fp8_empty_tile(const Fp8Job<TD>& j, int64_t ldc, int64_t ldd) {
@@ -508,7 +508,7 @@ FX_DEV void fp8_empty_tile(const Fp8Job<TD>& j, int64_t ldc, int64_t ldd) {
         }
 }
 
-template <int AF, typename TD, typename Source>
+template <int AF, typename TD, bool NT, typename Source>
 __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
     extern __shared__ __align__(16) unsigned char smem[];
     typedef Fp8Loop<AF, TD, FP8_WALK_BM, FP8_WALK_BN, 2, 4> Loop;
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
         f32x16_t acc[Loop::TM][Loop::TN];
         loop.template run<true>(src.job(cur), src.job(nxt), buf0, buf1, par, acc);
         const Fp8Job<TD> j = src.job(cur);
-        fp8_epilogue<TD, Loop::TM, Loop::TN, true>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 4) * Loop::WM,
+        fp8_epilogue<TD, Loop::TM, Loop::TN, true, NT>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 4) * Loop::WM,
                                                    j.n0 + (loop.wave % 4) * Loop::WN, j.A.ext, j.B.ext,
                                                    smem + kFp8WalkStages + loop.wave * FP8_STAGE_BYTES, loop.lane);
         if (!more) break;
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
     f32x16_t acc[Loop::TM][Loop::TN];
     int par = 0;
     loop.template run<false>(j, j, smem, smem + Loop::STAGE, par, acc);
-    fp8_epilogue<TD, Loop::TM, Loop::TN, false>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 2) * Loop::WM,
+    fp8_epilogue<TD, Loop::TM, Loop::TN, false, false>(acc, j.C, src.ldc, j.D, src.ldd, j.m0 + (loop.wave / 2) * Loop::WM,
                                                 j.n0 + (loop.wave % 2) * Loop::WN, j.A.ext, j.B.ext,
                                                 smem + kFp8Tile128Stages + loop.wave * FP8_STAGE_BYTES, loop.lane);
 }
@@ -745,6 +745,7 @@ static inline bool fp8_scales_fit(int64_t rows, int64_t s_row, int64_t blocks, i
     return span < 2147483647.0;
 }
 constexpr int64_t kFp8MaxLd = (int64_t)1 << 23;
+constexpr int kFp8MaxExtent = 0x7fffffff - 512;      // a row number behind an edge tile stays an int
 
 // Rows of an operand start at 16-byte addresses.
 static inline bool fp8_bad_rows(const void* p, int64_t ld) { return !aligned16(p) || (ld & 15) != 0; }

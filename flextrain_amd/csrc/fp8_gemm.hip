@@ -105,47 +105,57 @@ static Fp8Plan fp8_plan(int M, int N, int K) {
 }
 
 template <int AF, typename TD, int MT, int NT>
-static void launch_small(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
+static int launch_small(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
     typedef Fp8Dense<TD, 16 * MT, 16 * NT> Source;
     typedef Fp8SmallShape<MT, NT> Shape;
     const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(a.ext, 16 * MT), fp8_cdiv(b.ext, 16 * NT)};
+    if (!grid_fits((int64_t)src.tiles_m * src.tiles_n, Shape::NW * 64)) FX_FAIL("fx_fp8_gemm: too many tiles");
     fp8_small_kernel<AF, TD, MT, NT, Shape::NW, Shape::U, Source><<<dim3((unsigned)(src.tiles_m * src.tiles_n)), Shape::NW * 64, 0, stream>>>(src);
+    return 0;
 }
 
 template <int AF, typename TD>
-static void launch_walk(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
+static int launch_walk(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, hipStream_t stream) {
     typedef Fp8Dense<TD, 256, 256> Source;
     const Source src{a, b, C, D, ldc, ldd, K, fp8_cdiv(a.ext, 256), fp8_cdiv(b.ext, 256)};
     const int64_t total = (int64_t)src.tiles_m * src.tiles_n;
+    if (total > 0x7fffffff) FX_FAIL("fx_fp8_gemm: too many tiles");
     const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
-    auto kern = fp8_walk_kernel<AF, TD, Source>;
-    FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
-    kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+    if ((size_t)a.ext * (size_t)b.ext * sizeof(TD) >= kFp8OnceBytes) {
+        auto kern = fp8_walk_kernel<AF, TD, true, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+    } else {
+        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+    }
+    FX_CHECK_LAUNCH("fx_fp8_gemm");
+    return 0;
 }
 
 template <int AF, typename TD>
 static int launch_dense(const Fp8View& a, const Fp8View& b, const TD* C, int64_t ldc, TD* D, int64_t ldd, int K, void* ws,
                         const Fp8Plan& p, hipStream_t stream) {
     const int M = a.ext, N = b.ext;
-    if (p.tile == 256) {
-        launch_walk<AF, TD>(a, b, C, ldc, D, ldd, K, stream);
-        FX_CHECK_LAUNCH("fx_fp8_gemm");
-        return 0;
-    }
+    if (p.tile == 256) return launch_walk<AF, TD>(a, b, C, ldc, D, ldd, K, stream);
     if (p.tile == 0) {
+        int rc = 0;
         switch (p.small) {
-            case 0: launch_small<AF, TD, 1, 1>(a, b, C, ldc, D, ldd, K, stream); break;
-            case 1: launch_small<AF, TD, 1, 2>(a, b, C, ldc, D, ldd, K, stream); break;
-            case 2: launch_small<AF, TD, 1, 4>(a, b, C, ldc, D, ldd, K, stream); break;
-            case 3: launch_small<AF, TD, 2, 2>(a, b, C, ldc, D, ldd, K, stream); break;
-            case 4: launch_small<AF, TD, 2, 4>(a, b, C, ldc, D, ldd, K, stream); break;
-            case 5: launch_small<AF, TD, 4, 2>(a, b, C, ldc, D, ldd, K, stream); break;
-            default: launch_small<AF, TD, 4, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 0: rc = launch_small<AF, TD, 1, 1>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 1: rc = launch_small<AF, TD, 1, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 2: rc = launch_small<AF, TD, 1, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 3: rc = launch_small<AF, TD, 2, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 4: rc = launch_small<AF, TD, 2, 4>(a, b, C, ldc, D, ldd, K, stream); break;
+            case 5: rc = launch_small<AF, TD, 4, 2>(a, b, C, ldc, D, ldd, K, stream); break;
+            default: rc = launch_small<AF, TD, 4, 4>(a, b, C, ldc, D, ldd, K, stream); break;
         }
+        if (rc != 0) return rc;
         FX_CHECK_LAUNCH("fx_fp8_gemm");
         return 0;
     }
     const int tiles_m = fp8_cdiv(M, 128), tiles_n = fp8_cdiv(N, 128);
+    if (!grid_fits((int64_t)tiles_m * tiles_n * p.splits, 256)) FX_FAIL("fx_fp8_gemm: too many tiles");
     if (p.splits <= 1) {
         const Fp8Dense<TD, 128, 128> src{a, b, C, D, ldc, ldd, K, tiles_m, tiles_n};
         auto kern = fp8_tile_kernel128<AF, TD, Fp8Dense<TD, 128, 128>>;
@@ -183,6 +193,7 @@ extern "C" int fx_fp8_gemm(const void* A, int64_t lda, int a_dt, const void* SA,
     if (M < 0 || N < 0 || K < 0) FX_FAIL("fx_fp8_gemm: bad shape %d x %d x %d", M, N, K);
     if (!is_fp8_dt(a_dt)) FX_FAIL("fx_fp8_gemm: unsupported 8-bit dtype enum %d", a_dt);
     if (d_dt != DT_F32 && d_dt != DT_F16 && d_dt != DT_BF16) FX_FAIL("fx_fp8_gemm: unsupported output dtype enum %d", d_dt);
+    if (M > kFp8MaxExtent || N > kFp8MaxExtent) FX_FAIL("fx_fp8_gemm: too many rows");
     if (M == 0 || N == 0) return 0;
     if (!D || (K > 0 && (!A || !B || !SA || !SB))) FX_FAIL("fx_fp8_gemm: null pointer");
     if (K > 0 && (fp8_bad_rows(A, lda) || fp8_bad_rows(B, ldb))) FX_FAIL("fx_fp8_gemm: rows of A and B must start at 16-byte addresses");
@@ -191,7 +202,6 @@ extern "C" int fx_fp8_gemm(const void* A, int64_t lda, int a_dt, const void* SA,
     const int kb = fp8_cdiv(K, FP8_BK);
     if (!fp8_scales_fit(a_tiles ? fp8_cdiv(M, 128) : M, sa_row, kb, sa_k) || !fp8_scales_fit(b_tiles ? fp8_cdiv(N, 128) : N, sb_row, kb, sb_k))
         FX_FAIL("fx_fp8_gemm: a scale tensor must span less than 2 GB, with no negative stride");
-    if ((int64_t)fp8_cdiv(M, 16) * fp8_cdiv(N, 16) > 0x7fffffff) FX_FAIL("fx_fp8_gemm: too many tiles");
     if (ws_bytes < fx_fp8_gemm_ws_bytes(M, N, K) || (ws && !aligned16(ws)) || (!ws && fx_fp8_gemm_ws_bytes(M, N, K) > 0))
         FX_FAIL("fx_fp8_gemm: workspace missing, misaligned or too small");
     const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, a_tiles ? 7 : 0, M};

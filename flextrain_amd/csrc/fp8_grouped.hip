@@ -120,7 +120,7 @@ static int launch_rows_small(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
     typedef Fp8GroupedRows<TD, SHIFT, 16 * NT> Source;
     typedef Fp8SmallShape<MT, NT> Shape;
     const int tiles_n = fp8_cdiv(g.b.ext, 16 * NT);
-    if (g.most(SHIFT) * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
+    if (!grid_fits(g.most(SHIFT) * tiles_n, Shape::NW * 64)) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
     fp8_small_kernel<AF, TD, MT, NT, Shape::NW, Shape::U, Source><<<dim3((unsigned)(g.most(SHIFT) * tiles_n)), Shape::NW * 64, 0, stream>>>(g.template source<Source>(tiles_n));
     return 0;
 }
@@ -132,9 +132,15 @@ static int launch_rows_walk(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
     const int64_t total = g.most(8) * tiles_n;
     if (total > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
     const unsigned grid = (unsigned)(total < fp8_walk_grid() ? total : fp8_walk_grid());
-    auto kern = fp8_walk_kernel<AF, TD, Source>;
-    FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
-    kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(g.template source<Source>(tiles_n));
+    if ((size_t)g.rows * (size_t)g.b.ext * sizeof(TD) >= kFp8OnceBytes) {
+        auto kern = fp8_walk_kernel<AF, TD, true, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(g.template source<Source>(tiles_n));
+    } else {
+        auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(g.template source<Source>(tiles_n));
+    }
     return 0;
 }
 
@@ -147,7 +153,7 @@ static int launch_rows(const Fp8RowsArgs<TD>& g, hipStream_t stream) {
     } else if (p.shift == 7) {
         typedef Fp8GroupedRows<TD, 7, 128> Source;
         const int tiles_n = fp8_cdiv(g.b.ext, 128);
-        if (g.most(7) * tiles_n > 0x7fffffff) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
+        if (!grid_fits(g.most(7) * tiles_n, 256)) FX_FAIL("fx_fp8_grouped_gemm: too many tiles");
         auto kern = fp8_tile_kernel128<AF, TD, Source>;
         FX_ENSURE_DYNAMIC_LDS(kern, kFp8Tile128Lds);
         kern<<<dim3((unsigned)(g.most(7) * tiles_n)), 256, kFp8Tile128Lds, stream>>>(g.template source<Source>(tiles_n));
@@ -173,13 +179,18 @@ static int launch_wgrad(const Fp8View& a, const Fp8View& b, const int32_t* count
     const int M = a.ext, N = b.ext;
     const int64_t big = (int64_t)E * fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
     if (big >= 192) {
-        if (big > 0x7fffffff) FX_FAIL("fx_fp8_grouped_wgrad: too many tiles");
         typedef Fp8GroupedWgrad<TD, 256, 256> Source;
         const Source src{a, b, counts, C, D, ldc, ldd, c_expert, d_expert, capacity, E, fp8_cdiv(M, 256), fp8_cdiv(N, 256)};
         const unsigned grid = (unsigned)(big < fp8_walk_grid() ? big : fp8_walk_grid());
-        auto kern = fp8_walk_kernel<AF, TD, Source>;
-        FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
-        kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+        if ((size_t)E * (size_t)M * (size_t)N * sizeof(TD) >= kFp8OnceBytes) {
+            auto kern = fp8_walk_kernel<AF, TD, true, Source>;
+            FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+            kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+        } else {
+            auto kern = fp8_walk_kernel<AF, TD, false, Source>;
+            FX_ENSURE_DYNAMIC_LDS(kern, kFp8WalkLds);
+            kern<<<dim3(grid), 512, kFp8WalkLds, stream>>>(src);
+        }
     } else {
         const int64_t tiles = (int64_t)E * fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
         typedef Fp8GroupedWgrad<TD, 128, 128> Source;
@@ -205,6 +216,7 @@ extern "C" int fx_fp8_grouped_gemm(const void* A, int64_t lda, int a_dt, const v
     if (!is_fp8_dt(a_dt)) FX_FAIL("fx_fp8_grouped_gemm: unsupported 8-bit dtype enum %d", a_dt);
     if (d_dt != DT_F32 && d_dt != DT_F16 && d_dt != DT_BF16) FX_FAIL("fx_fp8_grouped_gemm: unsupported output dtype enum %d", d_dt);
     if (total_rows > (1 << 24)) FX_FAIL("fx_fp8_grouped_gemm: at most 2^24 expert rows");
+    if (N > kFp8MaxExtent) FX_FAIL("fx_fp8_grouped_gemm: too many rows of B");
     if (total_rows == 0 || N == 0) return 0;
     if (!counts || !D || (K > 0 && (!A || !B || !SA || !SB))) FX_FAIL("fx_fp8_grouped_gemm: null pointer");
     if (K > 0 && (fp8_bad_rows(A, lda) || fp8_bad_rows(B, ldb) || (b_expert & 15))) FX_FAIL("fx_fp8_grouped_gemm: rows of A and B must start at 16-byte addresses");
@@ -230,6 +242,7 @@ extern "C" int fx_fp8_grouped_wgrad(const void* A, int64_t lda, int a_dt, const 
     if (!is_fp8_dt(a_dt)) FX_FAIL("fx_fp8_grouped_wgrad: unsupported 8-bit dtype enum %d", a_dt);
     if (d_dt != DT_F32 && d_dt != DT_F16 && d_dt != DT_BF16) FX_FAIL("fx_fp8_grouped_wgrad: unsupported output dtype enum %d", d_dt);
     if (capacity >= kFp8MaxLd) FX_FAIL("fx_fp8_grouped_wgrad: at most 2^23 expert rows");
+    if (M > kFp8MaxExtent || N > kFp8MaxExtent) FX_FAIL("fx_fp8_grouped_wgrad: too many rows");
     if (M == 0 || N == 0) return 0;
     if (!counts || !D || (capacity > 0 && (!A || !B || !SA || !SB))) FX_FAIL("fx_fp8_grouped_wgrad: null pointer");
     if (capacity > 0 && (fp8_bad_rows(A, lda) || fp8_bad_rows(B, ldb))) FX_FAIL("fx_fp8_grouped_wgrad: rows of A and B must start at 16-byte addresses");
@@ -237,7 +250,7 @@ extern "C" int fx_fp8_grouped_wgrad(const void* A, int64_t lda, int a_dt, const 
     if (lda >= kFp8MaxLd || ldb >= kFp8MaxLd) FX_FAIL("fx_fp8_grouped_wgrad: row strides must be below 2^23 bytes");
     if (!fp8_scales_fit(M, sa_row, capacity / 128, sa_k) || !fp8_scales_fit(N, sb_row, capacity / 128, sb_k))
         FX_FAIL("fx_fp8_grouped_wgrad: a scale tensor must span less than 2 GB, with no negative stride");
-    if ((int64_t)E * fp8_cdiv(M, 128) * fp8_cdiv(N, 128) > 0x7fffffff) FX_FAIL("fx_fp8_grouped_wgrad: too many tiles");
+    if ((double)E * fp8_cdiv(M, 128) * fp8_cdiv(N, 128) > 2147483647.0) FX_FAIL("fx_fp8_grouped_wgrad: too many tiles");
     const Fp8View a{(const uint8_t*)A, (const uint8_t*)SA, (int)lda, (int)sa_row, (int)sa_k, 0, M};
     const Fp8View b{(const uint8_t*)B, (const uint8_t*)SB, (int)ldb, (int)sb_row, (int)sb_k, 0, N};
     int rc = -1;

@@ -385,6 +385,23 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_generic_kernel(
     DWOUT[col] = (TDW)acc;
 }
 
+// The same over bands of rows: partial sums of band b in row b of Y, which rmsnorm_dw_reduce_kernel adds up (one thread a
+// column over all rows waits on memory once a row: 16384 x 1001 bf16 4430 us, in bands 28 us).
+template <typename T>
+__global__ __launch_bounds__(256) void rmsnorm_dw_bands_kernel(const T* __restrict__ DY, const T* __restrict__ X, const float* __restrict__ RSTD,
+                                                               float* __restrict__ PARTIAL, int64_t rows, int ncols, int band) {
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= ncols) return;
+    const int64_t r0 = (int64_t)blockIdx.y * band, r1 = min(rows, r0 + band);
+    float acc = 0.f;
+#pragma unroll 8
+    for (int64_t r = r0; r < r1; ++r) acc += (float)DY[r * ncols + col] * ((float)X[r * ncols + col] * RSTD[r]);
+    PARTIAL[(int64_t)blockIdx.y * ncols + col] = acc;
+}
+// at most 512 bands, of 8 rows at least
+static inline int dw_band(int64_t rows) { return (int)(rows <= 4096 ? 8 : (rows + 511) / 512); }
+static inline int dw_bands(int64_t rows) { return (int)((rows + dw_band(rows) - 1) / dw_band(rows)); }
+
 struct NormCfg { int lpr, maxv; };
 
 static inline bool pick_cfg(int ncols, NormCfg& c) {
@@ -490,8 +507,16 @@ extern "C" size_t fx_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols) {
     return (size_t)bwd_grid(rows, groups) * (size_t)ncols * sizeof(float);
 }
 
-// dx = (old ? old : 0) + the norm's gradient; old may be dx itself or another buffer
-static int rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd, void* dx, const void* old, void* dw,
+extern "C" size_t fx_add_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols) {
+    if (rows <= 0 || ncols <= 0) return 0;
+    // either path of rmsnorm_bwd: which one is taken depends on the tensors' addresses too
+    const size_t bands = (size_t)dw_bands(rows) * (size_t)ncols * sizeof(float), packs = fx_rmsnorm_bwd_ws_bytes(rows, ncols);
+    return bands > packs ? bands : packs;
+}
+
+// dx = (old ? old : 0) + the norm's gradient; old may be dx itself or another buffer.  banded: widths and addresses that
+// the vector kernel does not take sum dw over bands of rows in ws (fx_add_rmsnorm_bwd_ws_bytes) instead of row by row.
+static int rmsnorm_bwd(bool banded, const void* dy, const void* x, const void* w, const float* rstd, void* dx, const void* old, void* dw,
                        int dw_dt, int accumulate_dw, void* y_out, int64_t rows, int ncols, int x_dt, int w_dt, float* ws,
                        size_t ws_bytes, hipStream_t stream) {
     if (rows < 0 || ncols <= 0) FX_FAIL("fx_rmsnorm_bwd: bad shape rows=%lld ncols=%d", (long long)rows, ncols);
@@ -512,7 +537,19 @@ static int rmsnorm_bwd(const void* dy, const void* x, const void* w, const float
                 reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), w, w_dt, rstd,
                 reinterpret_cast<T*>(dx), reinterpret_cast<const T*>(old), reinterpret_cast<T*>(y_out), rows, ncols));
         FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dx)");
-        if (want_dw) {
+        if (want_dw && banded) {
+            const int band = dw_band(rows), bands = dw_bands(rows);
+            if (ws == nullptr || ws_bytes < (size_t)bands * (size_t)ncols * sizeof(float))
+                FX_FAIL("fx_add_rmsnorm_bwd: workspace too small (%zu bytes)", ws_bytes);
+            FX_DISPATCH_DTYPE(x_dt, T,
+                rmsnorm_dw_bands_kernel<T><<<dim3((unsigned)((ncols + 255) / 256), (unsigned)bands), 256, 0, stream>>>(
+                    reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), rstd, ws, rows, ncols, band));
+            FX_CHECK_LAUNCH("fx_add_rmsnorm_bwd(dw bands)");
+            FX_DISPATCH_DTYPE(dw_dt, TDW,
+                rmsnorm_dw_reduce_kernel<TDW><<<dim3((unsigned)((ncols + 31) / 32)), 256, 0, stream>>>(
+                    ws, bands, ncols, reinterpret_cast<TDW*>(dw), accumulate_dw));
+            FX_CHECK_LAUNCH("fx_add_rmsnorm_bwd(dw reduce)");
+        } else if (want_dw) {
             const unsigned grid = (unsigned)((ncols + 255) / 256);
             FX_DISPATCH_DTYPE(x_dt, T,
                 FX_DISPATCH_DTYPE(dw_dt, TDW,
@@ -545,12 +582,13 @@ extern "C" int fx_rmsnorm_bwd(const void* dy, const void* x, const void* w, cons
                               void* dx, int accumulate_dx, void* dw, int dw_dt, int accumulate_dw,
                               void* y_out, int64_t rows, int ncols, int x_dt, int w_dt,
                               float* ws, size_t ws_bytes, hipStream_t stream) {
-    return rmsnorm_bwd(dy, x, w, rstd, dx, accumulate_dx ? dx : nullptr, dw, dw_dt, accumulate_dw, y_out, rows, ncols,
+    return rmsnorm_bwd(false, dy, x, w, rstd, dx, accumulate_dx ? dx : nullptr, dw, dw_dt, accumulate_dw, y_out, rows, ncols,
                        x_dt, w_dt, ws, ws_bytes, stream);
 }
 
 extern "C" int fx_add_rmsnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx,
                                   void* dw, int dw_dt, int accumulate_dw, int64_t rows, int ncols, int x_dt, int w_dt,
                                   float* ws, size_t ws_bytes, hipStream_t stream) {
-    return rmsnorm_bwd(dy, h, w, rstd, dx, dh, dw, dw_dt, accumulate_dw, nullptr, rows, ncols, x_dt, w_dt, ws, ws_bytes, stream);
+    if (rows > 0xffffff) FX_FAIL("fx_add_rmsnorm_bwd: too many rows");      // (a launch has 2^32 threads at most)
+    return rmsnorm_bwd(true, dy, h, w, rstd, dx, dh, dw, dw_dt, accumulate_dw, nullptr, rows, ncols, x_dt, w_dt, ws, ws_bytes, stream);
 }

@@ -55,6 +55,12 @@ def _scale_store(batch, rows, blocks, device):
     return torch.empty((batch, blocks, rows), dtype=_E8M0, device=device).transpose(1, 2)
 
 
+def _extents(op, *sizes):
+    """Sizes that the C ABI takes as 32-bit integers."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError(f"{op}: a dimension is larger than 2**31 - 1")
+
+
 def _input_matrix(X, op):
     """(batch or None, rows, cols, row stride, batch stride) of a matrix to quantise."""
     shape, stride = X.shape, X.stride()
@@ -71,6 +77,8 @@ def _input_matrix(X, op):
         raise ValueError(f"{op}: the rows of X overlap")
     if len(shape) == 2:
         return None, rows, cols, ldx, 0
+    if shape[0] > 65535:
+        raise ValueError(f"{op}: a batch holds at most 65535 matrices")
     return shape[0], rows, cols, ldx, stride[0]
 
 
@@ -216,6 +224,10 @@ def _output(out, shape, out_dtype, C, device, op):
         ldc, c_batch = _addend(C, shape, out_dtype, "C", op)
     if out is not None:
         ldd, d_batch = _addend(out, shape, out_dtype, "out", op)
+        if len(shape) == 3 and shape[0] > 1 and not (
+                d_batch >= (shape[1] - 1) * ldd + shape[2]                                       # one behind the other
+                or (d_batch >= shape[2] and ldd >= (shape[0] - 1) * d_batch + shape[2])):        # side by side
+            raise ValueError(f"{op}: the experts' matrices in out overlap")
         return out, d_dt, ldd, d_batch, ldc, c_batch
     D = torch.empty(shape, dtype=out_dtype, device=device)
     return D, d_dt, shape[-1], shape[-1] * shape[-2], ldc, c_batch
@@ -231,13 +243,15 @@ def flextrain_fp8_matmul(A, A_scales, B, B_scales, C=None, out=None, out_dtype=N
 
     ``A`` is e4m3 or e5m2, ``B`` e4m3; each has scales per row and 128 k or per 128 x 128 tile (told apart by their
     shape).  ``C`` has the output's shape and dtype and may be ``out`` (a gradient accumulated in place).  Output
-    dtype: ``out_dtype``, else that of ``out`` or ``C``, else bf16."""
+    dtype: ``out_dtype``, else that of ``out`` or ``C``, else bf16.  Rows of ``A`` and ``B`` are less than 2**23 bytes
+    apart, and a scale tensor spans less than 2 GB."""
     op = "flextrain_fp8_matmul"
     a_shape, b_shape = A.shape, B.shape
     if len(a_shape) != 2 or len(b_shape) != 2 or a_shape[1] != b_shape[1]:
         raise ValueError(f"{op}: A {tuple(a_shape)} and B {tuple(b_shape)} must be (M, K) and (N, K)")
     a_dt = _operand_dtypes(A, B, op)
     (M, K), N = a_shape, b_shape[0]
+    _extents(op, M, N, K)
     kb = _blocks(K)
     lda, ldb = _values(A, M, K, A.stride(), "A", op), _values(B, N, K, B.stride(), "B", op)
     sa_row, sa_k, a_tiles = _scales(A_scales, M, kb, True, "A_scales", op)
@@ -262,7 +276,8 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
     ``A (rows, K)`` expert-sorted, e4m3 or e5m2, scales per row; ``B (E, N, K)`` e4m3, scales ``(E, ceil(N / 128),
     ceil(K / 128))`` (tiles) or ``(E, N, ceil(K / 128))``; ``counts (E,)`` int32 with the sum ``rows``.  With
     ``row_sources`` (int32, one entry per expert-sorted row) ``A`` is the unsorted matrix and its rows are gathered by
-    the tile loads.  Rows of ``out`` behind the last expert's are left as they were."""
+    the tile loads (it is then smaller than 4 GB).  At most 2**24 expert-sorted rows.  Rows of ``out`` behind the last
+    expert's are left as they were."""
     op = "flextrain_fp8_grouped_matmul"
     a_shape, b_shape = A.shape, B.shape
     if len(a_shape) != 2 or len(b_shape) != 3 or a_shape[1] != b_shape[2]:
@@ -270,6 +285,7 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
     a_dt = _operand_dtypes(A, B, op)
     E, N, K = b_shape
     a_rows, kb = a_shape[0], _blocks(K)
+    _extents(op, N, K)
     if _counts_of(counts, op) != E:
         raise ValueError(f"{op}: {counts.numel()} counts for {E} experts")
     rows = a_rows if row_sources is None else _sources_of(row_sources, op)
@@ -311,6 +327,7 @@ def flextrain_fp8_grouped_wgrad(A, A_scales, B, B_scales, counts, C=None, out=No
     a_dt = _operand_dtypes(A, B, op)
     E = _counts_of(counts, op)
     (M, cap), N = a_shape, b_shape[0]
+    _extents(op, M, N)
     if cap % 128:
         raise ValueError(f"{op}: the capacity {cap} is not a multiple of 128")
     if cap >= 1 << 23:

@@ -206,7 +206,7 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
         return dX, dW
     L = lib()
     with on_device(H):
-        nbytes = int(L.fx_rmsnorm_bwd_ws_bytes(T, D)) if dW is not None else 0
+        nbytes = int(L.fx_add_rmsnorm_bwd_ws_bytes(T, D)) if dW is not None else 0
         ws = torch.empty(nbytes // 4, dtype=torch.float32, device=H.device) if nbytes else None
         rc = L.fx_add_rmsnorm_bwd(ptr(dY), ptr(dH), ptr(H), ptr(W), ptr(rstd), ptr(dX), ptr(dW),
                                   dtype_enum(dW.dtype) if dW is not None else 0, 1 if accumulate else 0, T, D,
