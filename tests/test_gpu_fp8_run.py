@@ -204,7 +204,7 @@ class Step:
         put = lambda *shape, std=1.0, dtype=torch.bfloat16: (torch.randn(*shape, generator=g) * std).to(dtype).to(dev)
         self.x, self.res, self.wn = put(16, 512), put(16, 512), put(512)
         self.w = put(640, 512, std=0.05)
-        self.long = put(130, 9000), put(140, 9000)                                  # sliced contraction: a workspace
+        self.long = put(520, 9000), put(500, 9000)                                  # sliced contraction: a workspace
         self.many = put(1300, 300, std=0.1), put(2100, 300)
         self.ew = put(4, 200, 512, std=0.05)
         self.counts = torch.tensor([7, 0, 5, 4], dtype=torch.int32).to(dev)
