@@ -37,22 +37,23 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-def _fp8_rows(batch, rows, cols, dtype, device):
-    """Uninitialised 8-bit values ``(rows, cols)``, or ``(batch, rows, cols)`` when ``batch`` is not None, whose rows
-    start at multiples of 16 bytes."""
+def _fp8_rows(like, batch, rows, cols, dtype):
+    """Uninitialised 8-bit values ``(rows, cols)``, or ``(batch, rows, cols)`` when ``batch`` is not None, on the device of
+    ``like``, whose rows start at multiples of 16 bytes.  (``new_empty`` takes 0.4 us less than ``torch.empty`` with a
+    device.)"""
     ld = _round_up(cols, 16)
     if batch is None:
         if ld == cols:
-            return torch.empty((rows, cols), dtype=dtype, device=device)
-        return torch.empty((rows, ld), dtype=dtype, device=device)[:, :cols]
-    return torch.empty((batch, rows, ld), dtype=dtype, device=device)[..., :cols]
+            return like.new_empty((rows, cols), dtype=dtype)
+        return like.new_empty((rows, ld), dtype=dtype)[:, :cols]
+    return like.new_empty((batch, rows, ld), dtype=dtype)[..., :cols]
 
 
-def _scale_store(batch, rows, blocks, device):
+def _scale_store(like, batch, rows, blocks):
     """Uninitialised scales ``(rows, blocks)`` / ``(batch, rows, blocks)``, the block index outermost in memory."""
     if batch is None:
-        return torch.empty_strided((rows, blocks), (1, rows), dtype=_E8M0, device=device)
-    return torch.empty((batch, blocks, rows), dtype=_E8M0, device=device).transpose(1, 2)
+        return like.new_empty_strided((rows, blocks), (1, rows), dtype=_E8M0)
+    return like.new_empty((batch, blocks, rows), dtype=_E8M0).transpose(1, 2)
 
 
 def _extents(op, *sizes):
@@ -85,15 +86,15 @@ def _input_matrix(X, op):
 def _quantize(X, dtype, tiles, both, op):
     batch, rows, cols, ldx, x_batch = _input_matrix(X, op)
     require_same_device(X, op=op)
-    x_dt, q_dt, device = dtype_enum(X.dtype), fp8_enum(dtype), X.device
+    x_dt, q_dt = dtype_enum(X.dtype), fp8_enum(dtype)
     rb, cb = _blocks(rows), _blocks(cols)
     s_rows = rb if tiles else rows
-    q, s = _fp8_rows(batch, rows, cols, dtype, device), _scale_store(batch, s_rows, cb, device)
+    q, s = _fp8_rows(X, batch, rows, cols, dtype), _scale_store(X, batch, s_rows, cb)
     qt = st = None
     t_rows = 0
     if both:
         t_rows = cb if tiles else cols
-        qt, st = _fp8_rows(batch, cols, rows, dtype, device), _scale_store(batch, t_rows, rb, device)
+        qt, st = _fp8_rows(X, batch, cols, rows, dtype), _scale_store(X, batch, t_rows, rb)
     if rows == 0 or batch == 0:
         return q, s, qt, st
     ldq, ldt = _round_up(cols, 16), _round_up(rows, 16)
@@ -157,8 +158,8 @@ def flextrain_fp8_quantize_grouped_cols(X, counts, dtype=torch.float8_e4m3fn, ro
         raise ValueError(f"{op}: at most 2**24 expert rows")
     x_dt, q_dt = dtype_enum(X.dtype), fp8_enum(dtype)
     cap = (rows + 127 * E) // 128 * 128          # fx_fp8_grouped_capacity
-    qt = torch.empty((cols, cap), dtype=dtype, device=X.device)
-    st = _scale_store(None, cols, cap // 128, X.device)
+    qt = X.new_empty((cols, cap), dtype=dtype)
+    st = _scale_store(X, None, cols, cap // 128)
     if cap > 0:
         with on_device(X):
             rc = lib().fx_fp8_quantize_grouped_cols(X.data_ptr(), ldx, x_rows, rows, cols, x_dt, q_dt, counts.data_ptr(), E,
@@ -213,7 +214,7 @@ def _addend(t, shape, dtype, name, op):
     return stride[-2] if got[-2] > 1 else got[-1], stride[0]
 
 
-def _output(out, shape, out_dtype, C, device, op):
+def _output(like, out, shape, out_dtype, C, op):
     """(output, its dtype's enum, its row and batch strides, those of C): C and out have the output's shape and dtype."""
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else C.dtype if C is not None else torch.bfloat16
@@ -229,7 +230,7 @@ def _output(out, shape, out_dtype, C, device, op):
                 or (d_batch >= shape[2] and ldd >= (shape[0] - 1) * d_batch + shape[2])):        # side by side
             raise ValueError(f"{op}: the experts' matrices in out overlap")
         return out, d_dt, ldd, d_batch, ldc, c_batch
-    D = torch.empty(shape, dtype=out_dtype, device=device)
+    D = like.new_empty(shape, dtype=out_dtype)
     return D, d_dt, shape[-1], shape[-1] * shape[-2], ldc, c_batch
 
 
@@ -257,7 +258,7 @@ def flextrain_fp8_matmul(A, A_scales, B, B_scales, C=None, out=None, out_dtype=N
     sa_row, sa_k, a_tiles = _scales(A_scales, M, kb, True, "A_scales", op)
     sb_row, sb_k, b_tiles = _scales(B_scales, N, kb, True, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, C, out, op=op)
-    D, d_dt, ldd, _, ldc, _ = _output(out, (M, N), out_dtype, C, A.device, op)
+    D, d_dt, ldd, _, ldc, _ = _output(A, out, (M, N), out_dtype, C, op)
     if M == 0 or N == 0:
         return D
     with on_device(A):
@@ -302,7 +303,7 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
         raise ValueError(f"{op}: B_scales has shape {tuple(B_scales.shape)}, expected {E} experts")
     sb_row, sb_k, b_tiles = _scales(B_scales, N, kb, True, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, counts, row_sources, out, op=op)
-    D, d_dt, ldd, _, _, _ = _output(out, (rows, N), out_dtype, None, A.device, op)
+    D, d_dt, ldd, _, _, _ = _output(A, out, (rows, N), out_dtype, None, op)
     if rows == 0 or N == 0:
         return D
     with on_device(A):
@@ -336,7 +337,7 @@ def flextrain_fp8_grouped_wgrad(A, A_scales, B, B_scales, counts, C=None, out=No
     sa_row, sa_k, _ = _scales(A_scales, M, cap // 128, False, "A_scales", op)
     sb_row, sb_k, _ = _scales(B_scales, N, cap // 128, False, "B_scales", op)
     require_same_device(A, A_scales, B, B_scales, counts, C, out, op=op)
-    D, d_dt, ldd, d_batch, ldc, c_batch = _output(out, (E, M, N), out_dtype, C, A.device, op)
+    D, d_dt, ldd, d_batch, ldc, c_batch = _output(A, out, (E, M, N), out_dtype, C, op)
     if M == 0 or N == 0:
         return D
     with on_device(A):

@@ -145,7 +145,7 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     rounded on the way); ``None`` gives ``Y`` in ``X``'s dtype, equal to ``flextrain_rmsnorm_fwd(H, W)``, and no
     scales.  ``sum_out`` receives ``H`` and may be ``X`` or ``residual``."""
     op = "flextrain_add_rmsnorm_fwd"
-    shape, dtype, device = X.shape, X.dtype, X.device
+    shape, dtype = X.shape, X.dtype
     if len(shape) != 2 or not X.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
         _norm_config(X, W, None)            # raises
     T, D = shape
@@ -161,11 +161,11 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     H = sum_out
     if H is None:
         H = torch.empty_like(X) if residual is not None else X
-    rstd = torch.empty((T, 1), dtype=torch.float32, device=device)
+    rstd = X.new_empty((T, 1), dtype=torch.float32)
     if y_dt == x_dt:
         Y, scales, ldy = torch.empty_like(X), None, D
     else:
-        Y, scales = _fp8_rows(None, T, D, output_dtype, device), _scale_store(None, T, _blocks(D), device)
+        Y, scales = _fp8_rows(X, None, T, D, output_dtype), _scale_store(X, None, T, _blocks(D))
         ldy = _round_up(D, 16)
     with on_device(X):
         rc = lib().fx_add_rmsnorm_fwd(X.data_ptr(), None if residual is None else residual.data_ptr(),
