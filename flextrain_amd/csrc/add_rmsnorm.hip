@@ -22,10 +22,47 @@ FX_DEV float norm_w1(const void* w, int w_dt, int64_t c) {
     return w_dt == DT_F32 ? reinterpret_cast<const float*>(w)[c]
            : w_dt == DT_BF16 ? (float)reinterpret_cast<const bf16*>(w)[c] : (float)reinterpret_cast<const f16*>(w)[c];
 }
-FX_DEV void norm_w8(const void* w, int w_dt, int col, float (&o)[8]) {
-    if (w_dt == DT_F32) load_f32<float, 8>(reinterpret_cast<const float*>(w) + col, o);
-    else if (w_dt == DT_BF16) load_f32<bf16, 8>(reinterpret_cast<const bf16*>(w) + col, o);
-    else load_f32<f16, 8>(reinterpret_cast<const f16*>(w) + col, o);
+// Eight consecutive values of a row, at any address of their type.  TAIL: of the last pack of a row whose length is no
+// multiple of 8 only the first `left` exist (the others read as 0 and are not written).
+template <bool TAIL, typename T>
+FX_DEV void row_load8(const T* p, int left, float (&o)[8]) {
+    if (TAIL && left < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = j < left ? (float)p[j] : 0.f;
+        return;
+    }
+    typedef typename AnyPack<T>::type V;
+    constexpr int VN = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / VN; ++i) {
+        const V v = *reinterpret_cast<const V*>(p + i * VN);
+#pragma unroll
+        for (int j = 0; j < VN; ++j) o[i * VN + j] = (float)v[j];
+    }
+}
+template <bool TAIL, typename T>
+FX_DEV void row_store8(T* p, int left, const float (&x)[8]) {
+    if (TAIL && left < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = (T)x[j];
+        return;
+    }
+    typedef typename AnyPack<T>::type V;
+    constexpr int VN = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / VN; ++i) {
+        V v;
+#pragma unroll
+        for (int j = 0; j < VN; ++j) v[j] = (T)x[i * VN + j];
+        *reinterpret_cast<V*>(p + i * VN) = v;
+    }
+}
+template <bool TAIL>
+FX_DEV void norm_w8(const void* w, int w_dt, int col, int left, float (&o)[8]) {
+    if (w_dt == DT_F32) row_load8<TAIL>(reinterpret_cast<const float*>(w) + col, left, o);
+    else if (w_dt == DT_BF16) row_load8<TAIL>(reinterpret_cast<const bf16*>(w) + col, left, o);
+    else row_load8<TAIL>(reinterpret_cast<const f16*>(w) + col, left, o);
 }
 
 template <typename T, int OUT>
@@ -34,7 +71,7 @@ FX_DEV float normed(float h, float rstd, float w, bool has_w) {
     return (OUT == OUT_SAME ? round_to<T>(h * rstd) : h * rstd) * w;
 }
 
-template <typename T, int LPR, int MAXV, int OUT>
+template <typename T, int LPR, int MAXV, int OUT, bool TAIL>
 __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
                                                           T* H /* may alias X or R */, void* Y, int64_t ldy,
                                                           uint8_t* __restrict__ S, int64_t lds, float* __restrict__ RSTD,
@@ -51,14 +88,14 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
     for (int v = 0; v < MAXV; ++v) {
         const int col = (v * LPR + l) * 8;
         if (row_ok && col < ncols) {
-            load_f32<T, 8>(X + row * ncols + col, h[v]);
+            row_load8<TAIL>(X + row * ncols + col, ncols - col, h[v]);
             if (R != nullptr) {
                 float r[8];
-                load_f32<T, 8>(R + row * ncols + col, r);
+                row_load8<TAIL>(R + row * ncols + col, ncols - col, r);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[v][j] = round_to<T>(h[v][j] + r[j]);
             }
-            if (has_w) norm_w8(W, w_dt, col, w[v]);
+            if (has_w) norm_w8<TAIL>(W, w_dt, col, ncols - col, w[v]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[v][j] = 0.f;
@@ -80,12 +117,12 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
     for (int v = 0; v < MAXV; ++v) {
         const int col = (v * LPR + l) * 8;
         const bool ok = row_ok && col < ncols;
-        if (ok && H != nullptr) store_f32<T, 8>(H + row * ncols + col, h[v]);
+        if (ok && H != nullptr) row_store8<TAIL>(H + row * ncols + col, ncols - col, h[v]);
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = ok ? normed<T, OUT>(h[v][j], rstd, w[v][j], has_w) : 0.f;
+        for (int j = 0; j < 8; ++j) y[j] = ok && (!TAIL || col + j < ncols) ? normed<T, OUT>(h[v][j], rstd, w[v][j], has_w) : 0.f;
         if constexpr (OUT == OUT_SAME) {
-            if (ok) store_f32<T, 8>(reinterpret_cast<T*>(Y) + row * ldy + col, y);
+            if (ok) row_store8<TAIL>(reinterpret_cast<T*>(Y) + row * ldy + col, ncols - col, y);
         } else {
             unsigned m = 0;
 #pragma unroll
@@ -103,7 +140,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
     }
 }
 
-// Any width and alignment: one workgroup per row.  h is formed twice (for the statistics and for the output)
+// Rows longer than registers hold (16384): one workgroup per row.  h is formed twice (for the statistics and for the output)
 // from x and residual, element by element by the lane that later overwrites it, so H may alias either.
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
@@ -165,12 +202,15 @@ static void launch_add_rmsnorm(const void* x, const void* r, const void* w, int 
                                int64_t lds, float* rstd, int64_t rows, int ncols, float eps, hipStream_t stream) {
     const T *X = (const T*)x, *R = (const T*)r;
     T* H = (T*)h;
-    const bool vec = ncols % 8 == 0 && ncols <= 16384 && aligned16(x) && (!r || aligned16(r)) && (!w || aligned16(w)) &&
-                     (!h || aligned16(h)) && aligned16(y);
-#define GO(L, V)                                                                                              \
-    add_rmsnorm_kernel<T, L, V, OUT><<<dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), 256, 0, stream>>>( \
+#define GO_TAIL(L, V, TAIL_)                                                                                         \
+    add_rmsnorm_kernel<T, L, V, OUT, TAIL_><<<dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), 256, 0, stream>>>( \
         X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, eps)
-    if (!vec)
+#define GO(L, V)                                                                                                     \
+    do {                                                                                                             \
+        if (ncols % 8) GO_TAIL(L, V, true);                                                                          \
+        else GO_TAIL(L, V, false);                                                                                   \
+    } while (0)
+    if (ncols > 16384)
         add_rmsnorm_generic_kernel<T, OUT><<<dim3((unsigned)rows), 256, 0, stream>>>(X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, eps);
     else if (ncols <= 128) GO(16, 1);
     else if (ncols <= 256) GO(32, 1);
@@ -181,6 +221,7 @@ static void launch_add_rmsnorm(const void* x, const void* r, const void* w, int 
     else if (ncols <= 8192) GO(256, 4);
     else GO(256, 8);
 #undef GO
+#undef GO_TAIL
 }
 
 }  // namespace fx

@@ -133,34 +133,50 @@ FX_DEV unsigned cvt_pairs(unsigned p0, unsigned p1, int byte) {
     }
     return __builtin_bit_cast(unsigned, w);
 }
-// Eight consecutive 2-byte values of a row as four pairs, 0 behind its end.
-template <typename T, bool VEC, bool NT = false>
-FX_DEV void load4_pairs(const T* row, int64_t col, int64_t cols, unsigned (&o)[4]) {
-    if (VEC && col < cols) {
-        typedef unsigned u4_t __attribute__((ext_vector_type(4)));
-        const u4_t* p = reinterpret_cast<const u4_t*>(row + col);
-        const u4_t v = NT ? __builtin_nontemporal_load(p) : *p;
+// Vectors at any address of their element type: the card takes 16-byte accesses at any alignment, so rows of odd lengths
+// need no copies element by element.
+template <typename T> struct AnyPack { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
+typedef unsigned u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// Eight consecutive 2-byte values of a row that has `cols` of them as four pairs, 0 behind its end.  WHOLE: a lane's eight
+// lie in the row or behind its end together.
+template <typename T, bool WHOLE, bool NT>
+FX_DEV void load8(const T* row, int64_t col, int64_t cols, unsigned (&o)[4]) {
+    if constexpr (WHOLE) {
+        u32x4_any_t v = {0u, 0u, 0u, 0u};
+        if (col < cols) {
+            const u32x4_any_t* p = reinterpret_cast<const u32x4_any_t*>(row + col);
+            v = NT ? __builtin_nontemporal_load(p) : *p;
+        }
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = v[d];
     } else {
         const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            const unsigned lo = !VEC && col + 2 * d < cols ? p[col + 2 * d] : 0u, hi = !VEC && col + 2 * d + 1 < cols ? p[col + 2 * d + 1] : 0u;
+            const unsigned lo = col + 2 * d < cols ? p[col + 2 * d] : 0u, hi = col + 2 * d + 1 < cols ? p[col + 2 * d + 1] : 0u;
             o[d] = lo | (hi << 16);
         }
     }
 }
-
-// Eight consecutive values of a row that has `cols` of them, 0 behind its end.  VEC: the address is 16-byte
-// aligned and a pack never straddles the end.
-template <typename T, bool VEC, bool NT = false>
-FX_DEV void load8_or_zero(const T* row, int64_t col, int64_t cols, float (&o)[8]) {
-    if (VEC && col < cols) {
-        load_f32<T, 8, NT>(row + col, o);
+// The same of 4-byte values.
+template <bool WHOLE, bool NT>
+FX_DEV void load8(const float* row, int64_t col, int64_t cols, float (&o)[8]) {
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x4_any_t v = {0.f, 0.f, 0.f, 0.f};
+            if (col < cols) {
+                const f32x4_any_t* p = reinterpret_cast<const f32x4_any_t*>(row + col + 4 * u);
+                v = NT ? __builtin_nontemporal_load(p) : *p;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * u + e] = v[e];
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (!VEC && col + j < cols) ? (float)row[col + j] : 0.f;
+        for (int j = 0; j < 8; ++j) o[j] = col + j < cols ? row[col + j] : 0.f;
     }
 }
 

@@ -154,12 +154,13 @@ struct Fp8Loop {
         lds_lane = (unsigned)(r * FP8_BK + (((2 * h) ^ swz(r)) << 4));
     }
 
-    // A contraction (K = 0 mod 128, or K > 128) is walked in steps(K) >= 2 K-steps.  When K is no multiple of 128 the last
+    // A contraction is walked in steps(K) >= 2 K-steps.  When K is no multiple of 128 the last
     // step starts back(K) bytes early, so that it ends where the row's last 16-byte chunk ends and no load leaves the
-    // row; patch() then zeroes the bytes that belong to the step before and those behind K.  A contraction of 128 has a
-    // second step made of such bytes only.
+    // row; patch() then zeroes the bytes that belong to the step before and those behind K.  A contraction of 128 or less
+    // has a second step made of such bytes only; of one below 128, start<true>() zeroes what lies behind K in the first as well,
+    // and the chunks behind its last one are requested from there.
     static FX_DEV int steps(int K) { return max(2, (K + FP8_BK - 1) / FP8_BK); }
-    static FX_DEV int back(int K) { return steps(K) * FP8_BK - ((K + 15) & ~15); }
+    static FX_DEV int back(int K) { return steps(K) * FP8_BK - max(FP8_BK, (K + 15) & ~15); }
     // Zero what lies outside bytes [lo, hi) of the landed K-step in `buf`: every lane mends the chunks it loaded itself (its
     // loads have been waited for; a barrier follows).  lo is a multiple of 16.
     FX_DEV void patch(uint8_t* buf, int lo, int hi) const {
@@ -189,17 +190,18 @@ struct Fp8Loop {
         const int wm = wave / WAVES_N, wn = wave % WAVES_N;
         const int rr = lane >> 3, pos = lane & 7;
         const bool gathered = j.row_map != nullptr;
+        const int last = min(FP8_BK, (j.K + 15) & ~15) - 16;        // offset of a row's last chunk within a K-step
         // offsets are taken from the tile's first row (gathered: from the source's, which is below 4 GB)
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int r = (i * NW + wave) * 8 + rr;
             const int64_t row = a_row(j, r) - (gathered ? 0 : j.m0);
-            aoff[i] = (unsigned)(row * j.A.ld + ((pos ^ swz(r)) << 4));
+            aoff[i] = (unsigned)(row * j.A.ld + min((pos ^ swz(r)) << 4, last));
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int r = (i * NW + wave) * 8 + rr;
-            boff[i] = (unsigned)((int64_t)(min(j.n0 + r, j.B.ext - 1) - j.n0) * j.B.ld + ((pos ^ swz(r)) << 4));
+            boff[i] = (unsigned)((int64_t)(min(j.n0 + r, j.B.ext - 1) - j.n0) * j.B.ld + min((pos ^ swz(r)) << 4, last));
         }
         abase = j.A.p + (gathered ? 0 : (int64_t)j.m0 * j.A.ld);
         bbase = j.B.p + (int64_t)j.n0 * j.B.ld;
@@ -213,7 +215,9 @@ struct Fp8Loop {
         sbk = j.K > FP8_BK ? j.B.s_k : 0;
     }
 
-    // First tile of a workgroup: its first two K-steps requested, the first landed and readable by everyone.
+    // First tile of a workgroup: its first two K-steps requested, the first landed and readable by everyone.  SHORT: the
+    // contraction may be below 128.
+    template <bool SHORT>
     FX_DEV void start(const Fp8Job<TD>& j, uint8_t* buf0, uint8_t* buf1) {
         setup(j);
         fetch_scales();
@@ -221,6 +225,9 @@ struct Fp8Loop {
         move(steps(j.K) == 2 ? -back(j.K) : 0);
         issue(buf1);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LD) : "memory");
+        if constexpr (SHORT) {
+            if (j.K < FP8_BK) patch(buf0, 0, j.K);
+        }
         __syncthreads();
     }
 
@@ -389,6 +396,8 @@ struct Fp8Loop {
 // 593 us for the expert weight gradients, which move 1.6 GB of C and D.
 // LAND: before the first store, everything this wave has requested so far must have landed (loads and stores share one
 // counter: a wait placed after the stores would also wait for them to drain).
+// Rows of C and D may start at any address of their type (an output of 919 columns): the card takes 16-byte accesses there,
+// and the element by element form is left to a row's last chunk (10736 x 5921 x 1723 202 -> 123 us, against 8 two-byte stores a chunk).
 constexpr int FP8_STAGE_BYTES = 4096;      // per wave
 
 template <typename TD, int TM, int TN, bool LAND, bool NT>
@@ -400,8 +409,7 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
     constexpr int JP = sizeof(TD) == 2 ? TN : 1, PASS = TN / JP;
     constexpr int CB = sizeof(TD) == 2 ? TM : (TM + 1) / 2;  // bands whose C is requested together
     const int r = lane & 31, h = lane >> 5, rr = lane >> 3, ch = lane & 7;
-    const bool vec = (ldd % CE) == 0 && (reinterpret_cast<uintptr_t>(D) & 15u) == 0 &&
-                     (C == nullptr || ((ldc % CE) == 0 && (reinterpret_cast<uintptr_t>(C) & 15u) == 0));
+    typedef typename AnyPack<TD>::type Any;                  // rows of C and D start anywhere
     auto at = [&](int row, int c) { return reinterpret_cast<Pack*>(st + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
     Pack c[CB][PASS][4];
 #pragma unroll
@@ -416,8 +424,8 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
                         const int row = row_base + (i + b) * 32 + t * 8 + rr, col = col_base + s * 32 + ch * CE;
                         if (row < M) {
                             const TD* src = C + (int64_t)row * ldc + col;
-                            if (vec && col + CE <= N) {
-                                c[b][s][t] = NT ? __builtin_nontemporal_load(reinterpret_cast<const Pack*>(src)) : *reinterpret_cast<const Pack*>(src);
+                            if (col + CE <= N) {
+                                c[b][s][t] = NT ? __builtin_nontemporal_load(reinterpret_cast<const Any*>(src)) : *reinterpret_cast<const Any*>(src);
                             } else {
 #pragma unroll
                                 for (int e = 0; e < CE; ++e)
@@ -469,9 +477,9 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
                 const int row = row_base + i * 32 + t * 8 + rr, col = col_base + s * 32 + ch * CE;
                 if (row < M && col < N) {
                     TD* d = D + (int64_t)row * ldd + col;
-                    if (vec && col + CE <= N) {
-                        if (NT) __builtin_nontemporal_store(o, reinterpret_cast<Pack*>(d));
-                        else *reinterpret_cast<Pack*>(d) = o;
+                    if (col + CE <= N) {
+                        if (NT) __builtin_nontemporal_store((Any)o, reinterpret_cast<Any*>(d));
+                        else *reinterpret_cast<Any*>(d) = o;
                     } else {
 #pragma unroll
                         for (int e = 0; e < CE; ++e)
@@ -530,7 +538,7 @@ __global__ __launch_bounds__(512) void fp8_walk_kernel(Source src) {
     int id = blockIdx.x;
     typename Source::Where cur;
     if (!find(id, cur)) return;
-    loop.start(src.job(cur), buf0, buf1);
+    loop.template start<false>(src.job(cur), buf0, buf1);
     int par = 0;
     for (;;) {
         typename Source::Where nxt = cur;
@@ -567,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel128(Source src) {
         fp8_empty_tile<TD, 128, 128, 256>(j, src.ldc, src.ldd);
         return;
     }
-    loop.start(j, smem, smem + Loop::STAGE);
+    loop.template start<true>(j, smem, smem + Loop::STAGE);
     f32x16_t acc[Loop::TM][Loop::TN];
     int par = 0;
     loop.template run<false>(j, j, smem, smem + Loop::STAGE, par, acc);
@@ -676,18 +684,16 @@ __global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
         for (int n = 0; n < NT; ++n) red[wave][i * NT + n][lane] = acc[i][n];
     __syncthreads();
     // lane holds D[m = lane % 16][n = 4 (lane / 16) .. + 3] of a 16 x 16 block; wave t % NW finishes block t
-    const bool vec = (src.ldd & 3) == 0 && (reinterpret_cast<uintptr_t>(j.D) % (4 * sizeof(TD))) == 0 &&
-                     (j.C == nullptr || ((src.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(j.C) % (4 * sizeof(TD))) == 0));
     for (int t = wave; t < MT * NT; t += NW) {
         f32x4v_t s = red[0][t][lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) s += red[w][t][lane];
         const int m = j.m0 + (t / NT) * 16 + r, n = j.n0 + (t % NT) * 16 + h * 4;
         if (m >= j.A.ext) continue;
-        typedef TD t4_t __attribute__((ext_vector_type(4)));
+        typedef TD t4_t __attribute__((ext_vector_type(4), aligned(sizeof(TD))));       // (rows start anywhere)
         TD* d = j.D + (int64_t)m * src.ldd + n;
         const TD* c = j.C != nullptr ? j.C + (int64_t)m * src.ldc + n : nullptr;
-        if (vec && n + 4 <= j.B.ext) {
+        if (n + 4 <= j.B.ext) {
             if (c != nullptr) {
                 const t4_t cv = *reinterpret_cast<const t4_t*>(c);
 #pragma unroll

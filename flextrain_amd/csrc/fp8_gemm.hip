@@ -88,7 +88,7 @@ static Fp8Plan fp8_plan(int M, int N, int K) {
         const double t = fp8_time_small(c, (double)fp8_cdiv(M, 16 * c.mt), N, steps);
         if (t < t_best) { t_best = t; best = Fp8Plan{0, i, 1, K}; }
     }
-    if (K < FP8_BK) return best;                                    // (the tile loads want a whole block)
+    if (K == 0) return best;
     const double tiles = (double)fp8_cdiv(M, 128) * fp8_cdiv(N, 128);
     for (int want = 1; want <= 16; want *= 2) {
         const int slice = fp8_cdiv(steps, want) * FP8_BK;
@@ -96,11 +96,11 @@ static Fp8Plan fp8_plan(int M, int N, int K) {
         if (splits > 1 && K - (splits - 1) * slice < FP8_BK) --splits;      // the last slice takes what is short of a block
         if (splits != want && want > 1) break;
         if (want > 1 && (steps / want < 4 || tiles * splits > 512.0)) break;
-        double t = fp8_time_128(tiles * splits, (double)(slice / FP8_BK));
+        double t = fp8_time_128(tiles * splits, (double)(slice > FP8_BK ? slice / FP8_BK : 2));
         if (splits > 1) t += 5.0 + (double)M * N * 4.0 * (2 * splits + 1) / 4.0e6;
         if (t < t_best) { t_best = t; best = Fp8Plan{128, 0, splits, splits > 1 ? slice : K}; }
     }
-    if (fp8_time_256((double)fp8_cdiv(M, 256) * fp8_cdiv(N, 256), steps) < t_best) best = Fp8Plan{256, 0, 1, K};
+    if (K >= FP8_BK && fp8_time_256((double)fp8_cdiv(M, 256) * fp8_cdiv(N, 256), steps > 1 ? steps : 2) < t_best) best = Fp8Plan{256, 0, 1, K};
     return best;
 }
 

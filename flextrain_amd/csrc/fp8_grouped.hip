@@ -91,10 +91,9 @@ static Fp8RowsPlan fp8_rows_plan(int64_t rows, int E, int N, int K) {
         const double t = fp8_time_small(c, tiles(16 * c.mt), N, steps);
         if (t < t_best) { t_best = t; best = Fp8RowsPlan{c.mt == 1 ? 4 : c.mt == 2 ? 5 : 6, i}; }
     }
-    if (K < FP8_BK) return best;                    // (the tile loads want a whole block)
-    const double t128 = fp8_time_128(tiles(128) * fp8_cdiv(N, 128), steps);
+    const double t128 = fp8_time_128(tiles(128) * fp8_cdiv(N, 128), steps > 1 ? steps : 2);
     if (t128 < t_best) { t_best = t128; best = Fp8RowsPlan{7, 0}; }
-    if (fp8_time_256(tiles(256) * fp8_cdiv(N, 256), steps) < t_best) best = Fp8RowsPlan{8, 0};
+    if (K >= FP8_BK && fp8_time_256(tiles(256) * fp8_cdiv(N, 256), steps > 1 ? steps : 2) < t_best) best = Fp8RowsPlan{8, 0};
     return best;
 }
 

@@ -8,6 +8,8 @@
 // contiguous, so one form of the matrix kernel serves them all.
 // Scales are stored with the block index of the contraction outermost (row index contiguous): the tile loader
 // of the product reads the scales of 32 consecutive rows at one k block as 32 consecutive bytes.
+#include <type_traits>
+
 #include "fp8.h"
 #include "flexhip.h"
 
@@ -22,7 +24,7 @@ struct QuantBatch {
 template <typename T, int FMT>
 struct Lane8 {            // 4-byte types
     float x[8];
-    template <bool VEC, bool NT> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load8_or_zero<T, VEC, NT>(row, col, cols, x); }
+    template <bool WHOLE, bool NT> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load8<WHOLE, NT>(row, col, cols, x); }
     FX_DEV unsigned mag() const {
         unsigned m = 0;
 #pragma unroll
@@ -40,7 +42,7 @@ struct Lane8 {            // 4-byte types
 template <typename T, int FMT>
 struct Lane8Pairs {       // 2-byte types
     unsigned x[4];
-    template <bool VEC, bool NT> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load4_pairs<T, VEC, NT>(row, col, cols, x); }
+    template <bool WHOLE, bool NT> FX_DEV void load(const T* row, int64_t col, int64_t cols) { load8<T, WHOLE, NT>(row, col, cols, x); }
     FX_DEV unsigned block_mag() const {
         unsigned m = pk_umax(pk_umax(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu), pk_umax(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
         m = max(m & 0xffffu, m >> 16);
@@ -58,7 +60,7 @@ template <int FMT> struct LaneOf<float, FMT> { typedef Lane8<float, FMT> type; }
 // Rows form.  A workgroup takes 16 rows x 512 columns: a wave 4 rows, one after the other, its 64 lanes
 // covering 4 blocks of 128 columns (1 KB of bf16 per load instruction).  A 16-lane group ends with the scale
 // bytes of 4 consecutive rows, which leave as one 4-byte store.
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q,
                                                        int64_t ldq, uint8_t* __restrict__ S, int64_t lds, int64_t rows,
                                                        int64_t cols, unsigned tiles_c, QuantBatch batch) {
@@ -69,11 +71,16 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ X, 
     const int64_t tr = blockIdx.x / tiles_c, tc = blockIdx.x % tiles_c;
     const int64_t row0 = tr * 16 + wave * 4, col = tc * 512 + lane * 8;
     typename LaneOf<T, FMT>::type x[4];
+    // (the last columns of rows whose length is no multiple of 8 are read one by one)
+    auto load = [&](auto whole) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int64_t r = row0 + u;
-        x[u].template load<VEC, false>(X + (r < rows ? r : 0) * ldx, col, r < rows ? cols : 0);
-    }
+        for (int u = 0; u < 4; ++u) {
+            const int64_t r = row0 + u;
+            x[u].template load<decltype(whole)::value, false>(X + (r < rows ? r : 0) * ldx, col, r < rows ? cols : 0);
+        }
+    };
+    if (tc * 512 + 512 <= cols || (cols & 7) == 0) load(std::true_type());
+    else load(std::false_type());
     unsigned bytes = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -100,7 +107,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ X, 
 //                  and full 128-byte runs of a transposed row leave 16 bytes per lane
 // ROWS / COLS: which outputs are written; TILE: one scale for all 128 x 128 values.
 // GROUPED: the row axis is the expert-padded order (find_group_tile), optionally gathered through MAP.
-template <typename T, int FMT, bool VEC, bool ROWS, bool COLS, bool TILE, bool GROUPED, bool NT = false>
+template <typename T, int FMT, bool ROWS, bool COLS, bool TILE, bool GROUPED, bool NT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 6 : 3) void fp8_tile_kernel(
     const T* __restrict__ X, int64_t ldx, uint8_t* __restrict__ Q, int64_t ldq, uint8_t* __restrict__ S, int64_t lds,
     uint8_t* __restrict__ QT, int64_t ldt, uint8_t* __restrict__ ST, int64_t ldst, int64_t rows, int64_t cols,
@@ -128,15 +135,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 6 : 3) void fp8_tile_kernel(
     typedef typename LaneOf<T, FMT>::type Lane;
     constexpr bool PAIRS = sizeof(T) == 2;
     Lane x[8];
+    auto load = [&](auto whole) {
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        const int r = g * 8 + p;
-        const bool ok = r < live;
-        int64_t src = ok ? first + r : 0;
-        // a map entry outside the source must not turn into an address outside it
-        if (GROUPED && MAP != nullptr && ok) src = min(max((int64_t)MAP[src], (int64_t)0), src_rows - 1);
-        x[p].template load<VEC, NT>(X + src * ldx, col, ok ? cols : 0);
-    }
+        for (int p = 0; p < 8; ++p) {
+            const int r = g * 8 + p;
+            const bool ok = r < live;
+            int64_t src = ok ? first + r : 0;
+            // a map entry outside the source must not turn into an address outside it
+            if (GROUPED && MAP != nullptr && ok) src = min(max((int64_t)MAP[src], (int64_t)0), src_rows - 1);
+            x[p].template load<decltype(whole)::value, NT>(X + src * ldx, col, ok ? cols : 0);
+        }
+    };
+    if (tc * 128 + 128 <= cols || (cols & 7) == 0) load(std::true_type());
+    else load(std::false_type());
     int tile_b = 0;
     if (TILE) {
         unsigned m = 0;
@@ -272,11 +283,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 6 : 3) void fp8_tile_kernel(
     }
 }
 
-// 16-byte packs: every row of x starts at a 16-byte address and its length is a whole number of 8-value packs
-static bool vec_rows(const void* x, int64_t ldx, int64_t cols, int x_dt) {
-    return aligned16(x) && (ldx * elem_size(x_dt)) % 16 == 0 && cols % 8 == 0;
-}
-
 }  // namespace fx
 
 using namespace fx;
@@ -305,15 +311,13 @@ extern "C" int fx_fp8_quantize(const void* x, int64_t ldx, int64_t x_batch, int 
         FX_FAIL("fx_fp8_quantize: rows of qt must start at 16-byte addresses and hold %lld values, its scales %lld", (long long)rows, (long long)cols);
     if (ldq - cols >= 16 || (qt && ldt - rows >= 16)) FX_FAIL("fx_fp8_quantize: the rows of q and qt are padded to the next multiple of 16, not further");
     if (batch > 1 && ((q_batch & 15) || (qt && (qt_batch & 15)))) FX_FAIL("fx_fp8_quantize: matrices of a batch must start at 16-byte addresses");
-    const bool vec = vec_rows(x, ldx, cols, x_dt) && (batch == 1 || (x_batch * elem_size(x_dt)) % 16 == 0);
     const QuantBatch qb{x_batch, q_batch, s_batch, qt_batch, st_batch};
     uint8_t *Q = (uint8_t*)q, *S = (uint8_t*)s, *QT = (uint8_t*)qt, *ST = (uint8_t*)st;
     if (!qt && !tiles) {
         const int64_t tc = (cols + 511) / 512, blocks = (rows + 15) / 16 * tc;
         if (!grid_fits(blocks, 256)) FX_FAIL("fx_fp8_quantize: too many blocks");
         FX_DISPATCH_DTYPE(x_dt, T, FX_DISPATCH_FP8(q_dt, FMT, {
-            if (vec) fp8_rows_kernel<T, FMT, true><<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, stream>>>((const T*)x, ldx, Q, ldq, S, lds, rows, cols, (unsigned)tc, qb);
-            else fp8_rows_kernel<T, FMT, false><<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, stream>>>((const T*)x, ldx, Q, ldq, S, lds, rows, cols, (unsigned)tc, qb);
+            fp8_rows_kernel<T, FMT><<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, stream>>>((const T*)x, ldx, Q, ldq, S, lds, rows, cols, (unsigned)tc, qb);
         }));
         FX_CHECK_LAUNCH("fx_fp8_quantize");
         return 0;
@@ -323,14 +327,14 @@ extern "C" int fx_fp8_quantize(const void* x, int64_t ldx, int64_t x_batch, int 
     // read past the caches, which then hold the bytes being written: 8192 x 14336 bf16 both ways 111 -> 105 us, 65536 x 1536
     // columns by expert 72 -> 62 us
     const bool nt = (size_t)batch * (size_t)rows * (size_t)cols * elem_size(x_dt) >= kStreamingBytes;
-#define FX_TILE(VEC_, COLS_, TILE_, NT_)                                                                           \
-    fp8_tile_kernel<T, FMT, VEC_, true, COLS_, TILE_, false, NT_><<<dim3(blocks, (unsigned)batch), 256, 0, stream>>>( \
+#define FX_TILE(COLS_, TILE_, NT_)                                                                                 \
+    fp8_tile_kernel<T, FMT, true, COLS_, TILE_, false, NT_><<<dim3(blocks, (unsigned)batch), 256, 0, stream>>>(    \
         (const T*)x, ldx, Q, ldq, S, lds, QT, ldt, ST, ldst, rows, cols, (unsigned)cb, nullptr, 0, nullptr, (int64_t)0, qb)
     FX_DISPATCH_DTYPE(x_dt, T, FX_DISPATCH_FP8(q_dt, FMT, {
-        if (!qt) { if (vec) FX_TILE(true, false, true, false); else FX_TILE(false, false, true, false); }
-        else if (tiles) { if (vec) FX_TILE(true, true, true, false); else FX_TILE(false, true, true, false); }
-        else if (vec && nt) FX_TILE(true, true, false, true);
-        else { if (vec) FX_TILE(true, true, false, false); else FX_TILE(false, true, false, false); }
+        if (!qt) FX_TILE(false, true, false);
+        else if (tiles) FX_TILE(true, true, false);
+        else if (nt) FX_TILE(true, false, true);
+        else FX_TILE(true, false, false);
     }));
 #undef FX_TILE
     FX_CHECK_LAUNCH("fx_fp8_quantize");
@@ -357,14 +361,13 @@ extern "C" int fx_fp8_quantize_grouped_cols(const void* x, int64_t ldx, int64_t 
     const int64_t cb = (cols + 127) / 128;
     if (!grid_fits(cap / 128 * cb, 256)) FX_FAIL("fx_fp8_quantize_grouped_cols: too many blocks");
     const unsigned blocks = (unsigned)(cap / 128 * cb);
-    const bool vec = vec_rows(x, ldx, cols, x_dt);
     // rows read once (gathered ones belong to several experts) pass the caches, which hold the bytes being written instead
     const bool nt = row_map == nullptr && (size_t)rows * (size_t)cols * elem_size(x_dt) >= kStreamingBytes;
-#define FX_TILE(VEC_, NT_)                                                                                         \
-    fp8_tile_kernel<T, FMT, VEC_, false, true, false, true, NT_><<<dim3(blocks), 256, 0, stream>>>(                \
+#define FX_TILE(NT_)                                                                                               \
+    fp8_tile_kernel<T, FMT, false, true, false, true, NT_><<<dim3(blocks), 256, 0, stream>>>(                      \
         (const T*)x, ldx, nullptr, (int64_t)0, nullptr, (int64_t)0, (uint8_t*)qt, ldt, (uint8_t*)st, ldst, rows, cols,  \
         (unsigned)cb, counts, E, row_map, src_rows, QuantBatch{0, 0, 0, 0, 0})
-    FX_DISPATCH_DTYPE(x_dt, T, FX_DISPATCH_FP8(q_dt, FMT, { if (vec && nt) FX_TILE(true, true); else if (vec) FX_TILE(true, false); else FX_TILE(false, false); }));
+    FX_DISPATCH_DTYPE(x_dt, T, FX_DISPATCH_FP8(q_dt, FMT, { if (nt) FX_TILE(true); else FX_TILE(false); }));
 #undef FX_TILE
     FX_CHECK_LAUNCH("fx_fp8_quantize_grouped_cols");
     return 0;

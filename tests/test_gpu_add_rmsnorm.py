@@ -55,6 +55,13 @@ def test_forward(dev, rows, cols, dtype):
             torch.testing.assert_close(Y.cpu().double(), y, rtol=1.5 * torch.finfo(dtype).eps + 2.0 ** -18, atol=1e-30 if dtype != torch.float16 else 2.0 ** -24)
 
 
+# a last pack of 1 .. 7 values at every width of the kernel, and rows at every address
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(33, 121), (18, 129), (9, 257), (9, 511), (5, 1023), (3, 2047), (2, 3001), (2, 4101), (2, 8191), (2, 8195), (1, 16383), (2, 16387)])
+def test_forward_at_odd_widths(dev, rows, cols, dtype):
+    test_forward(dev, rows, cols, dtype)
+
+
 @pytest.mark.parametrize("rows,cols", [(5, 128), (3, 4096), (2, 1000), (3, 7)])
 def test_same_dtype_output_is_the_norm_of_the_sum(dev, rows, cols):
     g = gen(2)

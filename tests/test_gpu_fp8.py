@@ -281,6 +281,63 @@ def test_grouped_matmul_large(dev, E, avg, n, k):
                 check(out[some], av[some] @ bv.t(), av[some], bv, what=f"expert {e}")
 
 
+# a contraction shorter than a block, in tiles: one K-step whose bytes behind K are zeroed
+@pytest.mark.parametrize("m,n,k", [(1900, 1801, 94), (2300, 1500, 16), (1700, 2100, 127), (3500, 1010, 1)])
+def test_matmul_short_contraction_large_output(dev, m, n, k):
+    g = gen(m)
+    some = some_rows(g, m)
+    x, w = values(g, m, k), values(g, n, k, sigma=0.5)
+    nan = torch.full((m, 144), 0x7F, dtype=torch.uint8, device=dev).view(E4M3)      # NaN behind the rows' ends
+    a, sa, av = operand(dev, x)
+    nan[:, :k] = a
+    b, sb, bv = operand(dev, w, tiles=True)
+    av = av[some]
+    ref = av @ bv.t()
+    check(ops.flextrain_fp8_matmul(nan[:, :k], sa, b, sb)[some], ref, av, bv)
+    c = values(g, m, n)
+    check(ops.flextrain_fp8_matmul(a, sa, b, sb, C=c.to(dev))[some], ref + c[some].double(), av, bv, c[some])
+    counts = torch.tensor([m // 2, 0, m - m // 2], dtype=torch.int32).to(dev)
+    bb, sbb = torch.stack([b.view(torch.uint8)] * 3).view(E4M3) if k % 16 == 0 else None, torch.stack([sb.contiguous().view(torch.uint8)] * 3).view(sb.dtype)
+    if bb is not None:
+        check(ops.flextrain_fp8_grouped_matmul(a, sa, bb, sbb, counts)[some], ref, av, bv)
+
+
+# rows of the output at every alignment: widths that are no multiple of 8, and an output that starts inside a row
+@pytest.mark.parametrize("t", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(5, 33, 256), (130, 131, 256), (700, 1285, 300)])
+def test_matmul_outputs_at_any_address(dev, m, n, k, t):
+    g = gen(n)
+    a, sa, av = operand(dev, values(g, m, k))
+    b, sb, bv = operand(dev, values(g, n, k, sigma=k ** -0.5))
+    ref = av @ bv.t()
+    c = values(g, m, n, sigma=float(ref.std())).to(t)
+    wide = torch.full((m, n + 10), 7.0, dtype=t, device=dev)
+    add = torch.zeros(m, n + 4, dtype=t, device=dev)
+    add[:, 1:n + 1] = c.to(dev)
+    for first in (1, 2, 5):
+        ops.flextrain_fp8_matmul(a, sa, b, sb, C=add[:, 1:n + 1], out=wide[:, first:first + n])
+        check(wide[:, first:first + n], ref + c.double(), av, bv, c)
+        assert (wide[:, :first] == 7.0).all() and (wide[:, first + n:] == 7.0).all()
+        wide.fill_(7.0)
+
+
+# input rows at every alignment
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_rows_at_any_address(dev, dtype):
+    g = gen(12)
+    x = values(g, 130, 700, dtype)
+    xd = x.to(dev)
+    for first, cols in ((1, 600), (3, 641), (0, 699), (5, 128), (2, 7)):
+        part = x[:, first:first + cols]
+        q, s, qt, st = ops.flextrain_fp8_quantize_both(xd[:, first:first + cols])
+        for got, want, scales, n in ((q, part, s, "rows"), (qt, part.t().contiguous(), st, "columns")):
+            value, scale = o.quantize(want, E4M3)
+            same(got, value, n)
+            same(scales, scale, n)
+        same(ops.flextrain_fp8_quantize(xd[:, first:first + cols], tiles=True)[0], o.quantize(part, E4M3, 128)[0], "tiles")
+        same(ops.flextrain_fp8_quantize(xd[:, first:first + cols], dtype=E5M2)[0], o.quantize(part, E5M2)[0], "rows")
+
+
 def test_matmul_tiles_on_both_sides_and_strides(dev):
     g = gen(3)
     x, w = values(g, 200, 384), values(g, 300, 384)
