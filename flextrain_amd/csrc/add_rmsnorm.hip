@@ -22,49 +22,6 @@ FX_DEV float norm_w1(const void* w, int w_dt, int64_t c) {
     return w_dt == DT_F32 ? reinterpret_cast<const float*>(w)[c]
            : w_dt == DT_BF16 ? (float)reinterpret_cast<const bf16*>(w)[c] : (float)reinterpret_cast<const f16*>(w)[c];
 }
-// Eight consecutive values of a row, at any address of their type.  TAIL: of the last pack of a row whose length is no
-// multiple of 8 only the first `left` exist (the others read as 0 and are not written).
-template <bool TAIL, typename T>
-FX_DEV void row_load8(const T* p, int left, float (&o)[8]) {
-    if (TAIL && left < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = j < left ? (float)p[j] : 0.f;
-        return;
-    }
-    typedef typename AnyPack<T>::type V;
-    constexpr int VN = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8 / VN; ++i) {
-        const V v = *reinterpret_cast<const V*>(p + i * VN);
-#pragma unroll
-        for (int j = 0; j < VN; ++j) o[i * VN + j] = (float)v[j];
-    }
-}
-template <bool TAIL, typename T>
-FX_DEV void row_store8(T* p, int left, const float (&x)[8]) {
-    if (TAIL && left < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) p[j] = (T)x[j];
-        return;
-    }
-    typedef typename AnyPack<T>::type V;
-    constexpr int VN = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8 / VN; ++i) {
-        V v;
-#pragma unroll
-        for (int j = 0; j < VN; ++j) v[j] = (T)x[i * VN + j];
-        *reinterpret_cast<V*>(p + i * VN) = v;
-    }
-}
-template <bool TAIL>
-FX_DEV void norm_w8(const void* w, int w_dt, int col, int left, float (&o)[8]) {
-    if (w_dt == DT_F32) row_load8<TAIL>(reinterpret_cast<const float*>(w) + col, left, o);
-    else if (w_dt == DT_BF16) row_load8<TAIL>(reinterpret_cast<const bf16*>(w) + col, left, o);
-    else row_load8<TAIL>(reinterpret_cast<const f16*>(w) + col, left, o);
-}
-
 template <typename T, int OUT>
 FX_DEV float normed(float h, float rstd, float w, bool has_w) {
     if (!has_w) return h * rstd;
@@ -95,7 +52,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[v][j] = round_to<T>(h[v][j] + r[j]);
             }
-            if (has_w) norm_w8<TAIL>(W, w_dt, col, ncols - col, w[v]);
+            if (has_w) row_w8<TAIL>(W, w_dt, col, ncols - col, w[v]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[v][j] = 0.f;

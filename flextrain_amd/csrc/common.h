@@ -64,6 +64,54 @@ FX_DEV void store_f32(T* __restrict__ p, const float (&in)[N]) {
     }
 }
 
+// Vectors at any address of their element type: the card takes 16-byte accesses at any alignment, so rows of odd lengths
+// need no copies element by element.
+template <typename T> struct AnyPack { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
+
+// Eight consecutive values of a row, at any address of their type.  TAIL: of the last pack of a row whose length is no
+// multiple of 8 only the first `left` exist (the others read as 0 and are not written).
+template <bool TAIL, typename T>
+FX_DEV void row_load8(const T* p, int left, float (&o)[8]) {
+    if (TAIL && left < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = j < left ? (float)p[j] : 0.f;
+        return;
+    }
+    typedef typename AnyPack<T>::type V;
+    constexpr int VN = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / VN; ++i) {
+        const V v = *reinterpret_cast<const V*>(p + i * VN);
+#pragma unroll
+        for (int j = 0; j < VN; ++j) o[i * VN + j] = (float)v[j];
+    }
+}
+template <bool TAIL, typename T>
+FX_DEV void row_store8(T* p, int left, const float (&x)[8]) {
+    if (TAIL && left < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) p[j] = (T)x[j];
+        return;
+    }
+    typedef typename AnyPack<T>::type V;
+    constexpr int VN = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / VN; ++i) {
+        V v;
+#pragma unroll
+        for (int j = 0; j < VN; ++j) v[j] = (T)x[i * VN + j];
+        *reinterpret_cast<V*>(p + i * VN) = v;
+    }
+}
+// The same of a norm's weight, whose dtype is known at run time (wave-uniform branch).
+template <bool TAIL>
+FX_DEV void row_w8(const void* w, int w_dt, int col, int left, float (&o)[8]) {
+    if (w_dt == DT_F32) row_load8<TAIL>(reinterpret_cast<const float*>(w) + col, left, o);
+    else if (w_dt == DT_BF16) row_load8<TAIL>(reinterpret_cast<const bf16*>(w) + col, left, o);
+    else row_load8<TAIL>(reinterpret_cast<const f16*>(w) + col, left, o);
+}
+
 // Round an fp32 value to T and back (the reference kernels round at a few
 // named points; this reproduces one such rounding).
 template <typename T> FX_DEV float round_to(float v) { return (float)(T)v; }

@@ -133,9 +133,6 @@ FX_DEV unsigned cvt_pairs(unsigned p0, unsigned p1, int byte) {
     }
     return __builtin_bit_cast(unsigned, w);
 }
-// Vectors at any address of their element type: the card takes 16-byte accesses at any alignment, so rows of odd lengths
-// need no copies element by element.
-template <typename T> struct AnyPack { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
 typedef unsigned u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 

@@ -155,7 +155,8 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_generic_kernel(
 // ---------------------------------------------------------------------------
 // Backward: dx (+ old dx), optional y, dW partials.
 // ---------------------------------------------------------------------------
-template <typename T, int LPR, int MAXV, int THREADS>
+// ANY: rows at any address and of any length (a last pack of 1 .. 7 values is read, and written, one by one).
+template <typename T, int LPR, int MAXV, int THREADS, bool ANY>
 __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
     const T* __restrict__ DY, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
     const float* __restrict__ RSTD, T* DX, const T* OLD /* added to dx; may be DX; or null */, T* __restrict__ YOUT,
@@ -179,7 +180,10 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
         const int col = (v * LPR + l) * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { w[v][j] = 1.f; dw[v][j] = 0.f; }
-        if (has_w && col < ncols) load_w8(W, w_dt, col, w[v]);
+        if (has_w && col < ncols) {
+            if constexpr (ANY) row_w8<true>(W, w_dt, col, ncols - col, w[v]);
+            else load_w8(W, w_dt, col, w[v]);
+        }
     }
 
     // Raw 16-byte packs of the NEXT iteration's x, dy and (when accumulating) old dx are requested
@@ -189,6 +193,17 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
     typedef typename VecOf<T>::type Pack;
     constexpr int PN = 8 / VecOf<T>::N;     // 16-byte packs per 8 elements
     Pack xr[MAXV][PN], dyr[MAXV][PN], oldr[MAXV][PN];
+    auto pack = [&](const T* p, int left) {
+        if constexpr (!ANY) return *reinterpret_cast<const Pack*>(p);
+        Pack v;
+        if (left >= VecOf<T>::N) {
+            v = *reinterpret_cast<const typename AnyPack<T>::type*>(p);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VecOf<T>::N; ++e) v[e] = e < left ? p[e] : (T)0.f;
+        }
+        return v;
+    };
     auto fetch = [&](int it) {
         const int64_t row = ((int64_t)it * gridDim.x + blockIdx.x) * G + g;
         const bool ok = row < rows;
@@ -198,9 +213,9 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
             if (ok && col < ncols) {
 #pragma unroll
                 for (int q = 0; q < PN; ++q) {
-                    xr[v][q] = *reinterpret_cast<const Pack*>(X + row * ncols + col + q * VecOf<T>::N);
-                    dyr[v][q] = *reinterpret_cast<const Pack*>(DY + row * ncols + col + q * VecOf<T>::N);
-                    if (accumulate_dx) oldr[v][q] = *reinterpret_cast<const Pack*>(OLD + row * ncols + col + q * VecOf<T>::N);
+                    xr[v][q] = pack(X + row * ncols + col + q * VecOf<T>::N, ncols - col - q * VecOf<T>::N);
+                    dyr[v][q] = pack(DY + row * ncols + col + q * VecOf<T>::N, ncols - col - q * VecOf<T>::N);
+                    if (accumulate_dx) oldr[v][q] = pack(OLD + row * ncols + col + q * VecOf<T>::N, ncols - col - q * VecOf<T>::N);
                 }
             }
         }
@@ -254,7 +269,8 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dx[j] = (float)old[v][j / VecOf<T>::N][j % VecOf<T>::N] + dx[j];
                 }
-                store8<T>(DX + row * ncols + col, dx);
+                if constexpr (ANY) row_store8<true>(DX + row * ncols + col, ncols - col, dx);
+                else store8<T>(DX + row * ncols + col, dx);
                 if (YOUT != nullptr) {
                     float y[8];
 #pragma unroll
@@ -292,7 +308,11 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
 #pragma unroll
         for (int v = 0; v < MAXV; ++v) {
             const int col = (v * LPR + l) * 8;
-            if (col < ncols) {
+            if (ANY) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (col + j < ncols) out[col + j] = dw[v][j];
+            } else if (col < ncols) {
                 float4* o = reinterpret_cast<float4*>(out + col);
                 o[0] = make_float4(dw[v][0], dw[v][1], dw[v][2], dw[v][3]);
                 o[1] = make_float4(dw[v][4], dw[v][5], dw[v][6], dw[v][7]);
@@ -385,8 +405,8 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_generic_kernel(
     DWOUT[col] = (TDW)acc;
 }
 
-// The same over bands of rows: partial sums of band b in row b of Y, which rmsnorm_dw_reduce_kernel adds up (one thread a
-// column over all rows waits on memory once a row: 16384 x 1001 bf16 4430 us, in bands 28 us).
+// The same over bands of rows: partial sums of band b in row b of PARTIAL, which rmsnorm_dw_reduce_kernel adds up (one
+// thread a column over all rows waits on memory once a row: 16384 x 1001 bf16 4430 us, in bands 28 us).
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_dw_bands_kernel(const T* __restrict__ DY, const T* __restrict__ X, const float* __restrict__ RSTD,
                                                                float* __restrict__ PARTIAL, int64_t rows, int ncols, int band) {
@@ -404,8 +424,8 @@ static inline int dw_bands(int64_t rows) { return (int)((rows + dw_band(rows) - 
 
 struct NormCfg { int lpr, maxv; };
 
-static inline bool pick_cfg(int ncols, NormCfg& c) {
-    if (ncols % 8 != 0 || ncols > 16384) return false;
+static inline bool pick_cfg(int ncols, NormCfg& c, bool any = false) {
+    if ((ncols % 8 != 0 && !any) || ncols > 16384) return false;
     if (ncols <= 128) c = {16, 1};
     else if (ncols <= 256) c = {32, 1};
     else if (ncols <= 512) c = {64, 1};
@@ -458,7 +478,7 @@ static int launch_fwd(const void* x, const void* w, int w_dt, void* y, float* rs
     return -1;
 }
 
-template <typename T>
+template <typename T, bool ANY>
 static int launch_bwd(const void* dy, const void* x, const void* w, int w_dt, const float* rstd,
                       void* dx, const void* old, void* yout, float* partial, int nblocks, int64_t rows,
                       int ncols, const NormCfg& c, hipStream_t s) {
@@ -472,7 +492,7 @@ static int launch_bwd(const void* dy, const void* x, const void* w, int w_dt, co
         constexpr int G = TH / L;                                                                 \
         const int iters = (int)((rows + (int64_t)nblocks * G - 1) / ((int64_t)nblocks * G));      \
         const size_t lds = sizeof(float) * (TH / 64 + (size_t)(G / 2) * L * V * 8);               \
-        rmsnorm_bwd_kernel<T, L, V, TH><<<nblocks, TH, lds, s>>>(DY, X, w, w_dt, rstd, DX, OLD, Y, partial, rows, ncols, iters); \
+        rmsnorm_bwd_kernel<T, L, V, TH, ANY><<<nblocks, TH, lds, s>>>(DY, X, w, w_dt, rstd, DX, OLD, Y, partial, rows, ncols, iters); \
         return 0;                                                                                 \
     }
     FX_BWD_CASE(16, 1, 1024) FX_BWD_CASE(32, 1, 1024) FX_BWD_CASE(64, 1, 1024) FX_BWD_CASE(64, 2, 512)
@@ -509,14 +529,15 @@ extern "C" size_t fx_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols) {
 
 extern "C" size_t fx_add_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols) {
     if (rows <= 0 || ncols <= 0) return 0;
-    // either path of rmsnorm_bwd: which one is taken depends on the tensors' addresses too
-    const size_t bands = (size_t)dw_bands(rows) * (size_t)ncols * sizeof(float), packs = fx_rmsnorm_bwd_ws_bytes(rows, ncols);
-    return bands > packs ? bands : packs;
+    NormCfg c;
+    const int parts = pick_cfg(ncols, c, true) ? bwd_grid(rows, bwd_threads(c) / c.lpr) : dw_bands(rows);
+    return (size_t)parts * (size_t)ncols * sizeof(float);
 }
 
-// dx = (old ? old : 0) + the norm's gradient; old may be dx itself or another buffer.  banded: widths and addresses that
-// the vector kernel does not take sum dw over bands of rows in ws (fx_add_rmsnorm_bwd_ws_bytes) instead of row by row.
-static int rmsnorm_bwd(bool banded, const void* dy, const void* x, const void* w, const float* rstd, void* dx, const void* old, void* dw,
+// dx = (old ? old : 0) + the norm's gradient; old may be dx itself or another buffer.  any: rows at any address and of any
+// length take the vector kernel (16384 x 1001 bf16 34 us, element by element 72), and rows that are too long for it
+// sum dw over bands of rows in ws; ws is then of fx_add_rmsnorm_bwd_ws_bytes.
+static int rmsnorm_bwd(bool any, const void* dy, const void* x, const void* w, const float* rstd, void* dx, const void* old, void* dw,
                        int dw_dt, int accumulate_dw, void* y_out, int64_t rows, int ncols, int x_dt, int w_dt, float* ws,
                        size_t ws_bytes, hipStream_t stream) {
     if (rows < 0 || ncols <= 0) FX_FAIL("fx_rmsnorm_bwd: bad shape rows=%lld ncols=%d", (long long)rows, ncols);
@@ -524,23 +545,22 @@ static int rmsnorm_bwd(bool banded, const void* dy, const void* x, const void* w
     if (!dy || !x || !rstd || !dx) FX_FAIL("fx_rmsnorm_bwd: null pointer");
     const bool want_dw = (w != nullptr && dw != nullptr);
     NormCfg c;
-    bool vec = pick_cfg(ncols, c) && aligned16(dy) && aligned16(x) && aligned16(dx) && (old == nullptr || aligned16(old)) &&
+    const bool vec = pick_cfg(ncols, c) && aligned16(dy) && aligned16(x) && aligned16(dx) && (old == nullptr || aligned16(old)) &&
                (y_out == nullptr || aligned16(y_out)) && (w == nullptr || aligned16(w));
-    if (vec && want_dw) {
-        const size_t need = fx_rmsnorm_bwd_ws_bytes(rows, ncols);
+    const bool odd = !vec && any && pick_cfg(ncols, c, true);
+    if ((vec || any) && want_dw) {
+        const size_t need = any ? fx_add_rmsnorm_bwd_ws_bytes(rows, ncols) : fx_rmsnorm_bwd_ws_bytes(rows, ncols);
         if (ws == nullptr || ws_bytes < need)
             FX_FAIL("fx_rmsnorm_bwd: workspace too small (%zu < %zu bytes)", ws_bytes, need);
     }
-    if (!vec) {
+    if (!vec && !odd) {
         FX_DISPATCH_DTYPE(x_dt, T,
             rmsnorm_bwd_generic_kernel<T><<<dim3((unsigned)rows), 256, 0, stream>>>(
                 reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), w, w_dt, rstd,
                 reinterpret_cast<T*>(dx), reinterpret_cast<const T*>(old), reinterpret_cast<T*>(y_out), rows, ncols));
         FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dx)");
-        if (want_dw && banded) {
+        if (want_dw && any) {
             const int band = dw_band(rows), bands = dw_bands(rows);
-            if (ws == nullptr || ws_bytes < (size_t)bands * (size_t)ncols * sizeof(float))
-                FX_FAIL("fx_add_rmsnorm_bwd: workspace too small (%zu bytes)", ws_bytes);
             FX_DISPATCH_DTYPE(x_dt, T,
                 rmsnorm_dw_bands_kernel<T><<<dim3((unsigned)((ncols + 255) / 256), (unsigned)bands), 256, 0, stream>>>(
                     reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), rstd, ws, rows, ncols, band));
@@ -564,8 +584,8 @@ static int rmsnorm_bwd(bool banded, const void* dy, const void* x, const void* w
     const int nblocks = bwd_grid(rows, groups);
     int rc = -1;
     FX_DISPATCH_DTYPE(x_dt, T,
-        rc = launch_bwd<T>(dy, x, w, w_dt, rstd, dx, old, y_out, want_dw ? ws : nullptr,
-                           nblocks, rows, ncols, c, stream));
+        rc = odd ? launch_bwd<T, true>(dy, x, w, w_dt, rstd, dx, old, y_out, want_dw ? ws : nullptr, nblocks, rows, ncols, c, stream)
+                 : launch_bwd<T, false>(dy, x, w, w_dt, rstd, dx, old, y_out, want_dw ? ws : nullptr, nblocks, rows, ncols, c, stream));
     if (rc != 0) FX_FAIL("fx_rmsnorm_bwd: no kernel for ncols=%d", ncols);
     FX_CHECK_LAUNCH("fx_rmsnorm_bwd");
     if (want_dw) {

@@ -7,6 +7,8 @@ into, a missing one is allocated and overwritten.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, raw_stream, require_gpu, require_same_device, stream_ptr
@@ -176,6 +178,11 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     return Y, scales, H, rstd
 
 
+@lru_cache(maxsize=4096)
+def _bwd_ws_bytes(T, D):
+    return int(lib().fx_add_rmsnorm_bwd_ws_bytes(T, D))
+
+
 def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
     """``(dX, dW)`` of :func:`flextrain_add_rmsnorm_fwd`: ``dX = dH + (gradient of the norm)`` is the gradient of ``X``
     and of ``residual`` alike.
@@ -184,33 +191,39 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
     unless it is given as ``dX`` too.  ``dY`` is the gradient of the unquantised output (the 8-bit rounding is passed
     straight through).  ``dW``: accumulated into when given, else a fresh fp32 gradient; ``None`` without ``W``."""
     op = "flextrain_add_rmsnorm_bwd"
-    T, D, _, _ = _norm_config(H, W, None)
-    for t, name in ((dY, "dY"), (dH, "dH"), (dX, "dX")):
-        if t is not None:
-            _check_like(t, H, name)
+    shape, dtype = H.shape, H.dtype
+    if len(shape) != 2 or not H.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
+        _norm_config(H, W, None)            # raises
+    T, D = shape
+    _check_like(dY, H, "dY")
+    if dH is not None:
+        _check_like(dH, H, "dH")
+    if dX is not None:
+        _check_like(dX, H, "dX")
     if rstd.numel() != T or not rstd.is_contiguous() or rstd.dtype != torch.float32:
         raise ValueError(f"rstd must be a contiguous float32 tensor of shape {(T, 1)}")
     if W is None and dW is not None:
         raise ValueError(f"{op}: dW without W")
-    if dW is not None and (tuple(dW.shape) != (D,) or not dW.is_contiguous()):
+    if dW is not None and (dW.shape != shape[1:] or not dW.is_contiguous()):
         raise ValueError(f"dW must be contiguous of shape {(D,)}")
     require_same_device(dY, H, W, rstd, dH, dX, dW, op=op)
+    x_dt = dtype_enum(dtype)
     if dX is None:
         dX = torch.empty_like(H)
     accumulate = dW is not None
     if W is not None and dW is None:
-        dW = torch.empty(D, dtype=torch.float32, device=H.device)
+        dW = H.new_empty((D,), dtype=torch.float32)
         if T == 0:
             dW.zero_()
     if T == 0:
         return dX, dW
-    L = lib()
     with on_device(H):
-        nbytes = int(L.fx_add_rmsnorm_bwd_ws_bytes(T, D)) if dW is not None else 0
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=H.device) if nbytes else None
-        rc = L.fx_add_rmsnorm_bwd(ptr(dY), ptr(dH), ptr(H), ptr(W), ptr(rstd), ptr(dX), ptr(dW),
-                                  dtype_enum(dW.dtype) if dW is not None else 0, 1 if accumulate else 0, T, D,
-                                  dtype_enum(H.dtype), dtype_enum(W.dtype) if W is not None else 0, ptr(ws), nbytes,
-                                  raw_stream(H))
+        nbytes = _bwd_ws_bytes(T, D) if dW is not None else 0
+        ws = H.new_empty((nbytes // 4,), dtype=torch.float32) if nbytes else None
+        rc = lib().fx_add_rmsnorm_bwd(dY.data_ptr(), None if dH is None else dH.data_ptr(), H.data_ptr(),
+                                      None if W is None else W.data_ptr(), rstd.data_ptr(), dX.data_ptr(),
+                                      None if dW is None else dW.data_ptr(), 0 if dW is None else dtype_enum(dW.dtype),
+                                      1 if accumulate else 0, T, D, x_dt, 0 if W is None else dtype_enum(W.dtype),
+                                      None if ws is None else ws.data_ptr(), nbytes, raw_stream(H))
     check(rc, "fx_add_rmsnorm_bwd")
     return dX, dW

@@ -143,6 +143,31 @@ def test_backward(dev, rows, cols, dtype):
     assert none is None
 
 
+# a last pack of 1 .. 7 values at every width of the kernel, rows at every address, and one that is too long for it
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(600, 1), (33, 121), (700, 129), (300, 257), (40, 511), (900, 1023), (3, 2047), (520, 3001), (2, 4101), (2, 8191), (1, 8195), (1, 16383), (30, 16387)])
+def test_backward_at_odd_widths(dev, rows, cols, dtype):
+    test_backward(dev, rows, cols, dtype)
+
+
+@pytest.mark.parametrize("cols", [256, 100])
+def test_rows_at_any_address(dev, cols):
+    """Contiguous tensors that start inside a larger one, one element further each."""
+    g = gen(11)
+    n = 5 * cols
+    x, r, dy, w = values(g, 5, cols), values(g, 5, cols), values(g, 5, cols), (1 + 0.1 * torch.randn(cols, generator=g)).to(torch.bfloat16)
+    put = lambda t, k: torch.cat([torch.zeros(k, dtype=t.dtype), t.flatten()]).to(dev)[k:].view(t.shape)
+    first = ops.flextrain_add_rmsnorm_fwd(x.to(dev), r.to(dev), w.to(dev), output_dtype=o.E4M3)
+    back = ops.flextrain_add_rmsnorm_bwd(dy.to(dev), first[2], w.to(dev), first[3], dH=x.to(dev))
+    for k in (1, 3):
+        X, R, DY, W = put(x, k), put(r, k + 1), put(dy, k + 2), put(w, k)
+        got = ops.flextrain_add_rmsnorm_fwd(X, R, W, output_dtype=o.E4M3, sum_out=X)
+        for a, b in zip(got, first):
+            assert torch.equal(a.float(), b.float())
+        dx, dw = ops.flextrain_add_rmsnorm_bwd(DY, X, W, got[3], dH=put(x, k))
+        assert torch.equal(dx, back[0]) and torch.equal(dw, back[1])
+
+
 def test_backward_against_differences(dev):
     """sum(c * y) of the fp32 forward, differenced: a step of 2^-6 leaves a curvature error of its square and an fp32
     error of 2^-22 / 2^-6 of the sum's magnitude."""
