@@ -22,25 +22,68 @@ FX_DEV float norm_w1(const void* w, int w_dt, int64_t c) {
     return w_dt == DT_F32 ? reinterpret_cast<const float*>(w)[c]
            : w_dt == DT_BF16 ? (float)reinterpret_cast<const bf16*>(w)[c] : (float)reinterpret_cast<const f16*>(w)[c];
 }
+// With an 8-bit output every value is that of the exact y, rounded once: the statistics are 64-bit, and y = h * rstd * w comes as a
+// sum of two fp32 numbers.  (An fp32 y that is off by an ulp falls on the wrong side of the middle between two 8-bit values once
+// in a few million, so that two programs which add a row's squares in another order differ by whole steps of 2^-3 there.)
+// 8192 x 4096 bf16 take 45 us in fp32, 51 like this and 55 with 64-bit products.  An output in the input's type keeps the
+// fp32 arithmetic of flextrain_rmsnorm_fwd.
+template <int OUT> struct NormMath { typedef double type; };
+template <> struct NormMath<OUT_SAME> { typedef float type; };
+
+template <int W>
+FX_DEV double group_sum(double v) {
+#pragma unroll
+    for (int off = W / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+FX_DEV float mean_of(float ss, int n, double) { return ss / (float)n; }
+FX_DEV double mean_of(double ss, int, double inv_n) { return ss * inv_n; }
+FX_DEV float inverse_root(float m) { return rsqrtf(m); }
+// The instruction's estimate (22 bits or more) and two Newton steps; 0 and infinity have none.
+FX_DEV double inverse_root(double m) {
+    double r = __builtin_amdgcn_rsq(m);
+    if (m > 0.0 && m < __builtin_huge_val()) {
+        r = r * (1.5 - 0.5 * m * r * r);
+        r = r * (1.5 - 0.5 * m * r * r);
+    }
+    return r;
+}
+// h * (hi + lo) * w to fp32 by rounding to odd: of the two neighbours of a value between them the one whose last bit is 1.  It lies on
+// the same side of every 8-bit value, and of every middle between two, as the value itself, so rounding it again gives what
+// rounding the value gives.  Products and their remainders by fma: off by 2^-45 of the value or less (while it is far from
+// fp32's subnormals).
+FX_DEV float product_odd(float h, float hi, float lo, float w) {
+#pragma clang fp contract(off)
+    const float p = h * hi, pe = fmaf(h, lo, fmaf(h, hi, -p));
+    const float y = p * w, ye = fmaf(pe, w, fmaf(p, w, -y));
+    const float s = y + ye, t = (y - s) + ye;
+    unsigned b = __builtin_bit_cast(unsigned, s);
+    const unsigned other = (b ^ __builtin_bit_cast(unsigned, t)) >> 31;          // 1: the value is nearer to 0 than s
+    if (t != 0.f && (b & 1u) == 0u) b += 1u - 2u * other;
+    return finite_mag(y) == 0u ? y : __builtin_bit_cast(float, b);               // (0, infinite, NaN)
+}
+FX_DEV float low_part(float, float) { return 0.f; }
+FX_DEV float low_part(double r, float hi) { return hi > 0.f && hi < __builtin_huge_valf() ? (float)(r - (double)hi) : 0.f; }
 template <typename T, int OUT>
-FX_DEV float normed(float h, float rstd, float w, bool has_w) {
-    if (!has_w) return h * rstd;
-    return (OUT == OUT_SAME ? round_to<T>(h * rstd) : h * rstd) * w;
+FX_DEV float normed(float h, float hi, float lo, float w, bool has_w) {
+    if constexpr (OUT != OUT_SAME) return product_odd(h, hi, lo, has_w ? w : 1.f);
+    else return has_w ? round_to<T>(h * hi) * w : h * hi;
 }
 
 template <typename T, int LPR, int MAXV, int OUT, bool TAIL>
 __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
                                                           T* H /* may alias X or R */, void* Y, int64_t ldy,
                                                           uint8_t* __restrict__ S, int64_t lds, float* __restrict__ RSTD,
-                                                          int64_t rows, int ncols, float eps) {
+                                                          int64_t rows, int ncols, double inv_n, float eps) {
     constexpr int G = 256 / LPR;
-    __shared__ float red[4];
+    typedef typename NormMath<OUT>::type M;
+    __shared__ M red[4];
     const int tid = threadIdx.x, g = tid / LPR, l = tid % LPR;
     const int64_t row = (int64_t)blockIdx.x * G + g;
     const bool row_ok = row < rows;
     const bool has_w = W != nullptr;
     float h[MAXV][8], w[MAXV][8];
-    float ss = 0.f;
+    M ss = 0;
 #pragma unroll
     for (int v = 0; v < MAXV; ++v) {
         const int col = (v * LPR + l) * 8;
@@ -58,7 +101,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
             for (int j = 0; j < 8; ++j) h[v][j] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += h[v][j] * h[v][j];
+        for (int j = 0; j < 8; ++j) ss += (M)h[v][j] * (M)h[v][j];
     }
     if constexpr (LPR <= 64) {
         ss = group_sum<LPR>(ss);
@@ -68,8 +111,9 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
         __syncthreads();
         ss = (red[0] + red[1]) + (red[2] + red[3]);
     }
-    const float rstd = rsqrtf(ss / (float)ncols + eps);
-    if (row_ok && l == 0) RSTD[row] = rstd;
+    const M rstd = inverse_root(mean_of(ss, ncols, inv_n) + (M)eps);
+    const float hi = (float)rstd, lo = low_part(rstd, hi);
+    if (row_ok && l == 0) RSTD[row] = hi;
 #pragma unroll
     for (int v = 0; v < MAXV; ++v) {
         const int col = (v * LPR + l) * 8;
@@ -77,7 +121,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
         if (ok && H != nullptr) row_store8<TAIL>(H + row * ncols + col, ncols - col, h[v]);
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = ok && (!TAIL || col + j < ncols) ? normed<T, OUT>(h[v][j], rstd, w[v][j], has_w) : 0.f;
+        for (int j = 0; j < 8; ++j) y[j] = ok && (!TAIL || col + j < ncols) ? normed<T, OUT>(h[v][j], hi, lo, w[v][j], has_w) : 0.f;
         if constexpr (OUT == OUT_SAME) {
             if (ok) row_store8<TAIL>(reinterpret_cast<T*>(Y) + row * ldy + col, ncols - col, y);
         } else {
@@ -102,8 +146,9 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
                                                                   T* H, void* Y, int64_t ldy, uint8_t* __restrict__ S, int64_t lds,
-                                                                  float* __restrict__ RSTD, int64_t rows, int ncols, float eps) {
-    __shared__ float red[4];
+                                                                  float* __restrict__ RSTD, int64_t rows, int ncols, double inv_n, float eps) {
+    typedef typename NormMath<OUT>::type M;
+    __shared__ M red[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const T* x = X + row * ncols;
@@ -111,21 +156,22 @@ __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, co
     // wave w takes blocks w, w + 4, ... of 128 columns; a lane the columns lane and lane + 64 of a block
     const int blocks = (ncols + 127) / 128;
     auto sum_at = [&](int c) { return r ? round_to<T>((float)x[c] + (float)r[c]) : (float)x[c]; };
-    float ss = 0.f;
+    M ss = 0;
     for (int b = wave; b < blocks; b += 4)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int c = b * 128 + u * 64 + lane;
             if (c < ncols) {
-                const float v = sum_at(c);
+                const M v = sum_at(c);
                 ss += v * v;
             }
         }
     ss = group_sum<64>(ss);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
-    const float rstd = rsqrtf(((red[0] + red[1]) + (red[2] + red[3])) / (float)ncols + eps);
-    if (tid == 0) RSTD[row] = rstd;
+    const M rstd = inverse_root(mean_of((red[0] + red[1]) + (red[2] + red[3]), ncols, inv_n) + (M)eps);
+    const float hi = (float)rstd, lo = low_part(rstd, hi);
+    if (tid == 0) RSTD[row] = hi;
     for (int b = wave; b < blocks; b += 4) {
         float y[2];
         unsigned m = 0;
@@ -135,7 +181,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, co
             y[u] = 0.f;
             if (c < ncols) {
                 const float v = sum_at(c);
-                y[u] = normed<T, OUT>(v, rstd, W ? norm_w1(W, w_dt, c) : 1.f, W != nullptr);
+                y[u] = normed<T, OUT>(v, hi, lo, W ? norm_w1(W, w_dt, c) : 1.f, W != nullptr);
                 if (H != nullptr) H[row * ncols + c] = (T)v;
                 m = max(m, finite_mag(y[u]));
                 if constexpr (OUT == OUT_SAME) reinterpret_cast<T*>(Y)[row * ldy + c] = (T)y[u];
@@ -161,14 +207,14 @@ static void launch_add_rmsnorm(const void* x, const void* r, const void* w, int 
     T* H = (T*)h;
 #define GO_TAIL(L, V, TAIL_)                                                                                         \
     add_rmsnorm_kernel<T, L, V, OUT, TAIL_><<<dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), 256, 0, stream>>>( \
-        X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, eps)
+        X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, eps)
 #define GO(L, V)                                                                                                     \
     do {                                                                                                             \
         if (ncols % 8) GO_TAIL(L, V, true);                                                                          \
         else GO_TAIL(L, V, false);                                                                                   \
     } while (0)
     if (ncols > 16384)
-        add_rmsnorm_generic_kernel<T, OUT><<<dim3((unsigned)rows), 256, 0, stream>>>(X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, eps);
+        add_rmsnorm_generic_kernel<T, OUT><<<dim3((unsigned)rows), 256, 0, stream>>>(X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, eps);
     else if (ncols <= 128) GO(16, 1);
     else if (ncols <= 256) GO(32, 1);
     else if (ncols <= 512) GO(64, 1);

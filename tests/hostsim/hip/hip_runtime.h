@@ -382,6 +382,8 @@ inline unsigned perm_b32(unsigned hi, unsigned lo, unsigned sel) {
 
 // gfx950 builtins the kernels use, by their documented meaning
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
+// (the instruction's estimate: the callers refine it)
+#define __builtin_amdgcn_rsq(x) ((double)(float)(1.0 / sqrt(x)))
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_readfirstlane(x) (x)          /* only ever applied to wave-uniform values */
 #define __builtin_amdgcn_wave_barrier() hostsim::sync_wave()

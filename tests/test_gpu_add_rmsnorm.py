@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import fp8 as o
-from tests.test_gpu_fp8 import values
+from tests.test_gpu_fp8 import same, values
 from tests.util import gen
 
 from flextrain_amd import ops
@@ -53,6 +53,22 @@ def test_forward(dev, rows, cols, dtype):
             Y, none, H, R = ops.flextrain_add_rmsnorm_fwd(x.to(dev), rd, wd)
             assert none is None and torch.equal(H.cpu(), h)
             torch.testing.assert_close(Y.cpu().double(), y, rtol=1.5 * torch.finfo(dtype).eps + 2.0 ** -18, atol=1e-30 if dtype != torch.float16 else 2.0 ** -24)
+
+
+# 64-bit statistics and one rounding: every 8-bit value and scale is that of the exact y
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(64, 4096), (300, 1001), (1000, 128), (3, 16390)])
+def test_8_bit_values_are_rounded_once(dev, rows, cols, dtype):
+    g = gen(rows)
+    x, r, w = values(g, rows, cols, dtype), values(g, rows, cols, dtype), (1 + 0.1 * torch.randn(cols, generator=g)).to(dtype)
+    for fmt in (o.E4M3, o.E5M2):
+        for weight in (w, None):
+            q, s, _, rstd = ops.flextrain_add_rmsnorm_fwd(x.to(dev), r.to(dev), None if weight is None else weight.to(dev), output_dtype=fmt)
+            _, root, y = o.add_rmsnorm(x, r, weight, float(torch.tensor(EPS)))
+            want, scale = o.quantize(y, fmt)
+            same(q, want, "values")
+            same(s, scale, "scales")
+            assert ((rstd.cpu().double() - root).abs() <= 2.0 ** -24 * root).all()
 
 
 # a last pack of 1 .. 7 values at every width of the kernel, and rows at every address
