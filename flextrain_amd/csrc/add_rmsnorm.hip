@@ -7,7 +7,7 @@
 // the 8-bit row written once (7 bytes an element for 2-byte types; a norm followed by a quantiser moves 11).
 // The sum h is rounded to T before anything uses it: the backward pass starts from the stored h, and the
 // statistics must be those of the row it sees.  With an 8-bit output y is NOT rounded to T on the way (one
-// rounding, from fp32); with output type T the product is rounded as flextrain_rmsnorm_fwd rounds it
+// rounding, from the exact value); with output type T the product is rounded as flextrain_rmsnorm_fwd rounds it
 // (T(h * rstd) * w), bit for bit the same as that op on h.
 // Thread mapping: that of rmsnorm.hip (LPR lanes a row, pack v of lane l holds columns (v * LPR + l) * 8 .. + 7),
 // so the 128 columns of a block lie in one pack of 16 consecutive lanes.

@@ -143,8 +143,8 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
 
     ``H = X + residual`` rounded to ``X``'s dtype (``X`` itself without a residual), ``rstd (T, 1)`` fp32 of ``H``,
     ``Y = H * rstd * W``.  ``output_dtype``: ``torch.float8_e4m3fn`` / ``torch.float8_e5m2`` give ``Y`` in 8 bits with
-    ``scales (T, ceil(D / 128))`` as :func:`flextrain_fp8_quantize` defines them (quantised from fp32: ``Y`` is not
-    rounded on the way); ``None`` gives ``Y`` in ``X``'s dtype, equal to ``flextrain_rmsnorm_fwd(H, W)``, and no
+    ``scales (T, ceil(D / 128))`` as :func:`flextrain_fp8_quantize` defines them (``Y`` is formed exactly and rounded
+    once); ``None`` gives ``Y`` in ``X``'s dtype, equal to ``flextrain_rmsnorm_fwd(H, W)``, and no
     scales.  ``sum_out`` receives ``H`` and may be ``X`` or ``residual``."""
     op = "flextrain_add_rmsnorm_fwd"
     shape, dtype = X.shape, X.dtype
