@@ -505,15 +505,36 @@ constexpr size_t kFp8WalkStages = 128 * 1024, kFp8WalkLds = kFp8WalkStages + 8 *
 // (8192 x 8192 x 8192, 134 MB: 387 -> 402 us; 8192 x 14336 x 4096, 235 MB: 363 -> 375 us).
 constexpr size_t kFp8OnceBytes = (size_t)256 << 20;
 
-// A tile whose contraction is empty: C, or zeros.
+// A tile whose contraction is empty: C (nothing to do where D is C), or zeros.  16 bytes a lane, all of C requested before the
+// first store: 93 experts of 720 x 280, 8 of them with a row, 116 us element by element, 27 like this.
 template <typename TD, int BM, int BN, int NT>
 FX_DEV void fp8_empty_tile(const Fp8Job<TD>& j, int64_t ldc, int64_t ldd) {
-    const int rows = min(BM, j.A.ext - j.m0), cols = min(BN, j.B.ext - j.n0);
-    for (int r = threadIdx.x / 64; r < rows; r += NT / 64)
-        for (int c = threadIdx.x % 64; c < cols; c += 64) {
-            const int64_t m = j.m0 + r, n = j.n0 + c;
-            j.D[m * ldd + n] = j.C != nullptr ? j.C[m * ldc + n] : (TD)0.f;
+    if (j.C == j.D && ldc == ldd) return;
+    typedef typename AnyPack<TD>::type Any;
+    constexpr int CE = 16 / (int)sizeof(TD), ROW = BN / CE, STEP = NT / ROW, BATCH = 8;
+    static_assert(NT % ROW == 0 && BM % (STEP * BATCH) == 0, "whole batches");
+    const int col = j.n0 + (threadIdx.x % ROW) * CE, row0 = j.m0 + threadIdx.x / ROW;
+    const bool whole = col + CE <= j.B.ext;
+    for (int r = 0; r < BM; r += STEP * BATCH) {
+        Any v[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const int64_t row = row0 + r + u * STEP;
+#pragma unroll
+            for (int e = 0; e < CE; ++e) v[u][e] = (TD)0.f;
+            if (j.C != nullptr && row < j.A.ext && whole) v[u] = *reinterpret_cast<const Any*>(j.C + row * ldc + col);
         }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const int64_t row = row0 + r + u * STEP;
+            if (row >= j.A.ext) continue;
+            if (whole) {
+                *reinterpret_cast<Any*>(j.D + row * ldd + col) = v[u];
+            } else {
+                for (int e = 0; col + e < j.B.ext; ++e) j.D[row * ldd + col + e] = j.C != nullptr ? j.C[row * ldc + col + e] : (TD)0.f;
+            }
+        }
+    }
 }
 
 template <int AF, typename TD, bool NT, typename Source>
@@ -710,8 +731,9 @@ __global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
 // ---------------------------------------------------------------- which kernel
 // Times in microseconds, fitted to sweeps of M in 1 .. 2048, N and K in 1000 .. 14336 (dense) and of 8 .. 65536 rows over
 // 128 experts (within 15 % of what was measured except where the weights' bytes bind every form alike):
-//   small   4 + max(1, workgroups / 256) * steps * (MT + NT) * 0.05      a CU takes in 40 KB of operands per us
-//   128     4 + steps * 0.62 up to one workgroup per CU, 0.95 at two, then 1.1 for every further 512
+//   small   4 + max(1, workgroups / 256) * steps * (MT + NT) * 0.05 + 5 for every million outputs      a CU takes in 40 KB of
+//           operands per us; its stores are 8 bytes a lane
+//   128     4 + steps * 0.62 up to one workgroup per CU, 0.95 at two, then steps * 1.1 + 3 for every further 512
 //   256     4 + rounds of 256 * (steps * 1.5 + 5)
 // steps: 128-long K-steps.  Examples (measured): 64 x 4096 x 4096 small 2 x 2 10.2, 128 15.4; 512 x 4096 x 4096 small 32.9,
 // 128 23.9, 256 41.5; 1024 x 14336 x 4096 128 76.6, 256 59.4.
@@ -719,14 +741,14 @@ struct Fp8Small { int mt, nt; };
 constexpr Fp8Small kFp8Small[] = {{1, 1}, {1, 2}, {1, 4}, {2, 2}, {2, 4}, {4, 2}, {4, 4}};
 constexpr int kFp8Smalls = sizeof(kFp8Small) / sizeof(kFp8Small[0]);
 
-static inline double fp8_time_small(const Fp8Small& c, double tiles_m, int N, int steps) {
+static inline double fp8_time_small(const Fp8Small& c, double tiles_m, double rows, int N, int steps) {
     const double w = tiles_m * (double)((N + 16 * c.nt - 1) / (16 * c.nt)) / 256.0;
-    return 4.0 + (w > 1.0 ? w : 1.0) * steps * (c.mt + c.nt) * 0.05;
+    return 4.0 + (w > 1.0 ? w : 1.0) * steps * (c.mt + c.nt) * 0.05 + rows * (double)N * 5e-6;
 }
 static inline double fp8_time_128(double workgroups, double steps) {
     if (workgroups <= 256.0) return 4.0 + steps * 0.62;
     if (workgroups <= 512.0) return 4.0 + steps * (0.62 + 0.33 * (workgroups / 256.0 - 1.0));
-    return 4.0 + ceil(workgroups / 512.0) * steps * 1.1;
+    return 4.0 + ceil(workgroups / 512.0) * (steps * 1.1 + 3.0);
 }
 static inline double fp8_time_256(double tiles, double steps) { return 4.0 + ceil(tiles / 256.0) * (steps * 1.5 + 5.0); }
 

@@ -60,17 +60,35 @@ struct Fp8Split {
     }
 };
 
-// D = sum of the slices (ascending: the same bits every run) + C
+// D = sum of the slices (ascending: the same bits every run) + C.  A lane owns four columns of a row.
 template <typename TD>
 __global__ __launch_bounds__(256) void fp8_split_reduce_kernel(const float* __restrict__ P, int splits, int M, int N, const TD* C,
                                                                int64_t ldc, TD* D, int64_t ldd) {
-    const int64_t total = (int64_t)M * N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += P[k * total + i];
-        const int64_t r = i / N, c = i % N;
-        if (C != nullptr) s += (float)C[r * ldc + c];
-        D[r * ldd + c] = (TD)s;
+    const int r = blockIdx.y * 4 + (threadIdx.x >> 6), c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    if (r >= M || c >= N) return;
+    const int64_t slice = (int64_t)M * N;
+    P += (int64_t)r * N + c;
+    D += r * ldd + c;
+    if (C != nullptr) C += r * ldc + c;
+    if (c + 4 <= N) {
+        typedef TD t4_t __attribute__((ext_vector_type(4), aligned(sizeof(TD))));
+        f32x4_any_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4_any_t*>(P + k * slice);
+        if (C != nullptr) {
+            const t4_t add = *reinterpret_cast<const t4_t*>(C);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += (float)add[e];
+        }
+        const t4_t o = {(TD)s[0], (TD)s[1], (TD)s[2], (TD)s[3]};
+        *reinterpret_cast<t4_t*>(D) = o;
+    } else {
+        for (int e = 0; c + e < N; ++e) {
+            float s = 0.f;
+            for (int k = 0; k < splits; ++k) s += P[k * slice + e];
+            if (C != nullptr) s += (float)C[e];
+            D[e] = (TD)s;
+        }
     }
 }
 
@@ -85,7 +103,7 @@ static Fp8Plan fp8_plan(int M, int N, int K) {
     for (int i = 0; i < kFp8Smalls; ++i) {
         const Fp8Small& c = kFp8Small[i];
         if (c.mt > 1 && 16 * c.mt >= 2 * M) continue;               // at least half of it would be padding
-        const double t = fp8_time_small(c, (double)fp8_cdiv(M, 16 * c.mt), N, steps);
+        const double t = fp8_time_small(c, (double)fp8_cdiv(M, 16 * c.mt), M, N, steps);
         if (t < t_best) { t_best = t; best = Fp8Plan{0, i, 1, K}; }
     }
     if (K == 0) return best;
@@ -169,9 +187,7 @@ static int launch_dense(const Fp8View& a, const Fp8View& b, const TD* C, int64_t
     FX_ENSURE_DYNAMIC_LDS(kern, kFp8Tile128Lds);
     kern<<<dim3((unsigned)(tiles_m * tiles_n * p.splits)), 256, kFp8Tile128Lds, stream>>>(src);
     FX_CHECK_LAUNCH("fx_fp8_gemm(slices)");
-    int64_t blocks = ((int64_t)M * N + 255) / 256;
-    if (blocks > 2048) blocks = 2048;
-    fp8_split_reduce_kernel<TD><<<dim3((unsigned)blocks), 256, 0, stream>>>((const float*)ws, p.splits, M, N, C, ldc, D, ldd);
+    fp8_split_reduce_kernel<TD><<<dim3((unsigned)fp8_cdiv(N, 256), (unsigned)fp8_cdiv(M, 4)), 256, 0, stream>>>((const float*)ws, p.splits, M, N, C, ldc, D, ldd);
     FX_CHECK_LAUNCH("fx_fp8_gemm(reduce)");
     return 0;
 }

@@ -88,7 +88,7 @@ static Fp8RowsPlan fp8_rows_plan(int64_t rows, int E, int N, int K) {
     for (int i = 0; i < kFp8Smalls; ++i) {
         const Fp8Small& c = kFp8Small[i];
         if (c.mt > 1 && 16 * c.mt >= 2 * avg) continue;
-        const double t = fp8_time_small(c, tiles(16 * c.mt), N, steps);
+        const double t = fp8_time_small(c, tiles(16 * c.mt), (double)rows, N, steps);
         if (t < t_best) { t_best = t; best = Fp8RowsPlan{c.mt == 1 ? 4 : c.mt == 2 ? 5 : 6, i}; }
     }
     const double t128 = fp8_time_128(tiles(128) * fp8_cdiv(N, 128), steps > 1 ? steps : 2);
