@@ -190,5 +190,5 @@ def activate():
         return torch.empty(span, **kwargs).as_strided(size, stride)
 
     torch.empty_strided = empty_strided
-    torch.Tensor.new_empty = lambda self, size, dtype=None: torch.empty(size, dtype=dtype or self.dtype)
+    torch.Tensor.new_empty = lambda self, *size, dtype=None, **kw: torch.empty(*size, dtype=dtype or self.dtype, **kw)
     torch.Tensor.new_empty_strided = lambda self, size, stride, dtype=None: empty_strided(size, stride, dtype=dtype or self.dtype)
