@@ -64,6 +64,14 @@ FX_DEV void store_f32(T* __restrict__ p, const float (&in)[N]) {
     }
 }
 
+// pid -> position in the logical order: XCD x (= pid % 8) walks positions [x*per, (x+1)*per).
+FX_DEV int xcd_band(int pid, int total) {
+    constexpr int XCDS = 8;
+    if (total < XCDS * 4) return pid;
+    const int per = total / XCDS, body = per * XCDS;
+    return pid < body ? (pid % XCDS) * per + pid / XCDS : pid;
+}
+
 // Vectors at any address of their element type: the card takes 16-byte accesses at any alignment, so rows of odd lengths
 // need no copies element by element.
 template <typename T> struct AnyPack { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };

@@ -122,7 +122,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 6 : 3) void fp8_tile_kernel(
     __shared__ unsigned tilemax[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int g = tid >> 4, c = tid & 15;
-    const int64_t tr = blockIdx.x / tiles_c, tc = blockIdx.x % tiles_c;
+    // Neighbouring tiles of a row on one XCD: 8192 x 14336 bf16 both ways 101 -> 95 us.  Expert columns are better off
+    // without (65536 x 1536: 63 us, in bands 69).
+    const int id = GROUPED ? (int)blockIdx.x : xcd_band((int)blockIdx.x, (int)gridDim.x);
+    const int64_t tr = id / (int)tiles_c, tc = id % (int)tiles_c;
     int64_t first = tr * 128;
     int live = (int)min((int64_t)128, rows - first);
     if (GROUPED) {

@@ -1007,12 +1007,4 @@ FX_DEV void tile_coords(int pid, int tiles_m, int tiles_n, int& tm, int& tn) {
     tn = (p % width) / gsz;
 }
 
-// pid -> position in the logical order: XCD x (= pid % 8) walks positions [x*per, (x+1)*per).
-FX_DEV int xcd_band(int pid, int total) {
-    constexpr int XCDS = 8;
-    if (total < XCDS * 4) return pid;
-    const int per = total / XCDS, body = per * XCDS;
-    return pid < body ? (pid % XCDS) * per + pid / XCDS : pid;
-}
-
 }  // namespace fx
