@@ -12,7 +12,7 @@ from functools import lru_cache
 import torch
 
 from .._lib import check, dtype_enum, fp8_enum, lib, on_device, ptr, raw_stream, require_gpu, require_same_device, stream_ptr
-from .fp8 import _fp8_rows, _round_up, _scale_store, _blocks
+from .fp8 import _blocks, _extents, _fp8_rows, _round_up, _scale_store
 
 
 def _norm_config(X, W, head_dim):
@@ -153,6 +153,7 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     T, D = shape
     if D == 0:
         raise ValueError(f"{op}: X has no columns")
+    _extents(op, D)
     if residual is not None:
         _check_like(residual, X, "residual")
     if sum_out is not None:
@@ -195,6 +196,7 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
     if len(shape) != 2 or not H.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
         _norm_config(H, W, None)            # raises
     T, D = shape
+    _extents(op, D)
     _check_like(dY, H, "dY")
     if dH is not None:
         _check_like(dH, H, "dH")

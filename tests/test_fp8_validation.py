@@ -153,6 +153,29 @@ def test_grouped_wgrad_of_nothing_is_a_no_op():
     assert _wgrad(M=0, A=None, D=None) == 0 and _wgrad(N=0, B=None, D=None) == 0
 
 
+def test_dimensions_past_32_bits_are_refused_by_the_wrappers():
+    """(The C ABI takes them as int; tensors without storage show it.)"""
+    from flextrain_amd import ops
+
+    big = 1 << 31
+    fp8 = lambda *shape: torch.empty(shape, dtype=torch.float8_e4m3fn, device="meta")
+    scales = lambda *shape: torch.empty(shape, dtype=torch.float8_e8m0fnu, device="meta")
+    counts = torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="larger than"):
+        ops.flextrain_fp8_matmul(fp8(big, 16), scales(big, 1), fp8(8, 16), scales(8, 1))
+    with pytest.raises(ValueError, match="larger than"):
+        ops.flextrain_fp8_grouped_matmul(fp8(8, 16), scales(8, 1), fp8(2, big, 16), scales(2, big, 1), counts)
+    with pytest.raises(ValueError, match="larger than"):
+        ops.flextrain_fp8_grouped_wgrad(fp8(big, 128), scales(big, 1), fp8(8, 128), scales(8, 1), counts)
+    x = torch.empty(1, big, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="larger than"):
+        ops.flextrain_add_rmsnorm_fwd(x)
+    with pytest.raises(ValueError, match="larger than"):
+        ops.flextrain_add_rmsnorm_bwd(x, x, None, torch.empty(1, 1, device="meta"))
+    with pytest.raises(ValueError, match="65535"):
+        ops.flextrain_fp8_quantize(torch.empty(1 << 16, 1, 16, dtype=torch.bfloat16, device="meta"))
+
+
 def test_only_the_two_8_bit_types_have_an_enum():
     assert fp8_enum(torch.float8_e4m3fn) == E4M3 and fp8_enum(torch.float8_e5m2) == E5M2
     for t in (torch.bfloat16, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz, torch.uint8):
