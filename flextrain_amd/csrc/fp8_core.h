@@ -156,7 +156,8 @@ struct Fp8Loop {
 
     // A contraction is walked in steps(K) >= 2 K-steps.  When K is no multiple of 128 the last
     // step starts back(K) bytes early, so that it ends where the row's last 16-byte chunk ends and no load leaves the
-    // row; patch() then zeroes the bytes that belong to the step before and those behind K.  A contraction of 128 or less
+    // row; patch() then zeroes the bytes that belong to the step before and those behind K (a K that ends inside the last
+    // chunk of its 128 needs no step back, and still has bytes behind it).  A contraction of 128 or less
     // has a second step made of such bytes only; of one below 128, start<true>() zeroes what lies behind K in the first as well,
     // and the chunks behind its last one are requested from there.
     static FX_DEV int steps(int K) { return max(2, (K + FP8_BK - 1) / FP8_BK); }
@@ -295,7 +296,7 @@ struct Fp8Loop {
         // of the next K-step are read and the loads of the one after go out.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         if constexpr (SHORT) {
-            if (lo > 0) patch(nxt, lo, hi);
+            if (lo > 0 || hi < FP8_BK) patch(nxt, lo, hi);
         }
         __syncthreads();
         // packed here, where nothing is in flight: a use further down would wait for the tile loads issued since
@@ -371,7 +372,7 @@ struct Fp8Loop {
             }
             if (AHEAD) setup(next);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (lo > 0) patch(stage(n - 1), lo, hi);
+            if (lo > 0 || hi < FP8_BK) patch(stage(n - 1), lo, hi);
             __syncthreads();
             if (AHEAD) {
                 issue(stage(n - 2));
