@@ -8,6 +8,11 @@ row, ``(ceil(rows / 128), ceil(cols / 128))`` for 128 x 128 tiles.  The quantise
 outermost and pads rows of values to multiples of 16 bytes; the products take scales of any strides and values whose
 rows start at 16-byte addresses.
 
+An operand may be a part of a wider matrix: the products load rows in whole 16-byte pieces, and bytes of a row's last
+piece that lie behind its end do not count, whatever they are (NaN too).  Such a piece starts inside the row at a
+16-byte address, so the up to 15 bytes read behind a tensor's last row, or behind a single one, lie in its own memory
+page; they need not be the tensor's.
+
 =================  ==========================================  =====================================================
  product            operands                                    made by
 =================  ==========================================  =====================================================

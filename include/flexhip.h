@@ -545,7 +545,9 @@ int fx_fp8_quantize_grouped_cols(const void* x, int64_t ldx, int64_t src_rows, i
                                  void* st, int64_t ldst, hipStream_t stream);
 
 /* D (M, N) = A (M, K) B (N, K)^T + C, accumulated in fp32.  A: a_dt e4m3 or e5m2, B e4m3; rows start at 16-byte
- * addresses, less than 2^23 bytes apart, and are read up to the next multiple of 16 (what lies behind K does not count).  The scale of row r and k block b is SA[(a_tiles ? r / 128 : r) * sa_row + b * sa_k], SB likewise.
+ * addresses, less than 2^23 bytes apart, and are read in whole 16-byte pieces: up to 15 bytes behind a row's end, the
+ * last row's among them, in the piece that the row ends in (never another page); what lies behind K does not count.
+ * The scale of row r and k block b is SA[(a_tiles ? r / 128 : r) * sa_row + b * sa_k], SB likewise.
  * C (or NULL) and D: dtype d_dt (0 / 1 / 2); C may be D.  ws: fx_fp8_gemm_ws_bytes bytes, 16-byte aligned (may be
  * NULL when that is 0); calls that may overlap need one each. */
 size_t fx_fp8_gemm_ws_bytes(int M, int N, int K);

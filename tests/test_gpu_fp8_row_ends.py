@@ -53,6 +53,25 @@ def test_long_contractions(dev, m, n, k, junk):
     assert torch.equal(out, ops.flextrain_fp8_matmul(a, sa, b, sb, out_dtype=torch.float32))
 
 
+# one contiguous row, and rows of which the last ends where its memory does: the other bytes of the last 16 are another tensor's
+@pytest.mark.parametrize("m,n,k", [(1, 16, 14330), (1, 300, 1003), (1, 1, 5), (20, 16, 14321), (3, 1, 250)])
+def test_memory_that_ends_with_the_last_row(dev, m, n, k):
+    def last(q):
+        rows, ld = q.shape[0], -(-k // 16) * 16
+        memory = torch.full((rows * ld,), 0x7F, dtype=torch.uint8, device=dev)
+        memory[:(rows - 1) * ld + k].as_strided((rows, k), (ld, 1)).copy_(q.view(torch.uint8))
+        if rows == 1:
+            return memory[:k].view(1, k).view(q.dtype)
+        return memory[:(rows - 1) * ld + k].as_strided((rows, k), (ld, 1)).view(q.dtype)
+
+    g = gen(k)
+    a, sa, av = operand(dev, values(g, m, k))
+    b, sb, bv = operand(dev, values(g, n, k, sigma=k ** -0.5))
+    out = ops.flextrain_fp8_matmul(last(a), sa, last(b), sb, out_dtype=torch.float32)
+    check(out, av @ bv.t(), av, bv)
+    assert torch.equal(out, ops.flextrain_fp8_matmul(a, sa, b, sb, out_dtype=torch.float32))
+
+
 # 256 x 256 tiles, several to a workgroup
 @pytest.mark.parametrize("junk", ["nan", "finite"])
 @pytest.mark.parametrize("k", [241, 250, 255, 383, 1148])
