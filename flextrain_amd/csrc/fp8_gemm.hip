@@ -1,6 +1,6 @@
 // Matrix products of 8-bit operands with a power-of-two scale per block of 128 (fp8.h), gfx950.
 //
-//   D[M,N] = sum over k blocks of 2^(ea[m,kb] + eb[n,kb]) * (A[m,kb] . B[n,kb])  + C[M,N]         fp32 accumulate
+//   D[M,N] = sum over k blocks of 2^(ea[m,kb] + eb[n,kb]) * (A[m,kb] . B[n,kb])  + C[M,N]         (sums: see below)
 //
 // Both operands have the contraction contiguous (A (M,K), B (N,K)), which the quantiser's row and transposed
 // outputs provide for the forward product, the input gradient and the weight gradient alike: one form of the tile
