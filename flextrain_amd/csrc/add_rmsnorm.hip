@@ -8,7 +8,10 @@
 // The sum h is rounded to T before anything uses it: the backward pass starts from the stored h, and the
 // statistics must be those of the row it sees.  With an 8-bit output y is NOT rounded to T on the way (one
 // rounding, from the exact value); with output type T the product is rounded as flextrain_rmsnorm_fwd rounds it
-// (T(h * rstd) * w), bit for bit the same as that op on h.
+// (T(h * rstd) * w): the same rstd as that op on h where it takes its vector kernel (ncols % 8 == 0, at most 16384, 16-byte
+// addresses; its other kernel adds the squares in another order), and the same y in bf16 and fp32.  In fp16 the compiler
+// turns a product and its conversion into one v_fma_mix, which rounds once, in some places of either kernel and not in
+// others: with a weight up to 5 values of 100,000 are a step apart.
 // Thread mapping: that of rmsnorm.hip (LPR lanes a row, pack v of lane l holds columns (v * LPR + l) * 8 .. + 7),
 // so the 128 columns of a block lie in one pack of 16 consecutive lanes.
 // Bound by memory: 8192 x 4096 bf16 with a residual 51 us, 4.6 TB/s; one row 4 us, which is latency.

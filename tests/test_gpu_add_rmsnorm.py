@@ -221,3 +221,39 @@ def test_refusals(dev):
             ops.flextrain_add_rmsnorm_bwd(x, H, None, rstd, **bad)
     with pytest.raises(ValueError):
         ops.flextrain_add_rmsnorm_bwd(x, H, None, rstd[:2])
+
+
+# one width for every split of a row over lanes and packs
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cols", [8, 128, 136, 256, 512, 1000, 1024, 2048, 4096, 8192, 16384])
+def test_same_dtype_output_has_the_bits_of_the_norm(dev, cols, dtype):
+    """In fp16 a product may be rounded to fp32 on its way to fp16, or not: each of the two roundings of Y then falls to one
+    of two neighbours, at most two steps in all (2^-24 each among the subnormals)."""
+    g = gen(cols)
+    x, r = values(g, 3, cols, dtype).to(dev), values(g, 3, cols, dtype).to(dev)
+    weight = (1 + 0.1 * torch.randn(cols, generator=g)).to(dev)
+    for w in (None, weight, weight.to(dtype)):
+        for res in (r, None):
+            Y, _, H, R = ops.flextrain_add_rmsnorm_fwd(x, res, w)
+            want, rstd = ops.flextrain_rmsnorm_fwd(H, w)
+            assert torch.equal(R, rstd)
+            if dtype == torch.float16:
+                torch.testing.assert_close(Y.double(), want.double(), rtol=2 * torch.finfo(dtype).eps, atol=2.0 ** -23)
+            else:
+                assert torch.equal(Y, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cols,first", [(7, 0), (1001, 0), (16392, 0), (16391, 0), (256, 1), (4096, 3)])
+def test_same_dtype_output_of_other_rows_differs_by_the_order_of_a_sum(dev, cols, first, dtype):
+    """Two orders of at most 16392 squares: 65 a lane and 8 levels of a tree at most, each addition off by 2^-24, so the
+    means are 146 * 2^-24 apart and rstd half of that and two roots' roundings (below 2^-17).  Y is rounded twice, and either
+    rounding may fall to the other side: two steps of the type."""
+    g = gen(cols)
+    flat = torch.cat([torch.zeros(first, dtype=dtype), values(g, 3, cols, dtype).flatten()]).to(dev)
+    x, w = flat[first:].view(3, cols), (1 + 0.1 * torch.randn(cols, generator=g)).to(dev)
+    Y, _, H, R = ops.flextrain_add_rmsnorm_fwd(x, None, w)
+    assert H is x
+    want, rstd = ops.flextrain_rmsnorm_fwd(x, w)
+    torch.testing.assert_close(R.double(), rstd.double(), rtol=2.0 ** -17, atol=0)
+    torch.testing.assert_close(Y.double(), want.double(), rtol=2 * torch.finfo(dtype).eps + 2.0 ** -16, atol=2.0 ** -23 if dtype == torch.float16 else 0)
