@@ -139,7 +139,7 @@ _SIGNATURES = {
                                    c_void_p]),
     "compute_buf_size": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_double, c_int]),
     "fx_add_rmsnorm_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                   c_int64, c_int, c_float, c_int, c_int, c_int, c_void_p]),
+                                   c_int64, c_int, c_double, c_int, c_int, c_int, c_void_p]),
     "fx_add_rmsnorm_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                    c_int64, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "fx_fp8_quantize": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_int64,

@@ -29,8 +29,9 @@ FX_DEV float norm_w1(const void* w, int w_dt, int64_t c) {
 // With an 8-bit output every value is that of the exact y, rounded once: the statistics are 64-bit, and y = h * rstd * w comes as a
 // sum of two fp32 numbers.  (An fp32 y that is off by an ulp falls on the wrong side of the middle between two 8-bit values once
 // in a few million, so that two programs which add a row's squares in another order differ by whole steps of 2^-3 there.)
-// 8192 x 4096 bf16 take 45 us in fp32, 51 like this and 55 with 64-bit products.  An output in the input's type keeps the
-// fp32 arithmetic of flextrain_rmsnorm_fwd.
+// 8192 x 4096 bf16 take 45 us in fp32, 51 like this and 55 with 64-bit products.  eps comes in 64 bits too: 1e-5 rounded to fp32
+// moves rstd by 6e-9 where the mean square is as small as that.  An output in the input's type keeps the fp32 arithmetic
+// (eps with it) of flextrain_rmsnorm_fwd.
 template <int OUT> struct NormMath { typedef double type; };
 template <> struct NormMath<OUT_SAME> { typedef float type; };
 
@@ -78,7 +79,7 @@ template <typename T, int LPR, int MAXV, int OUT, bool TAIL>
 __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
                                                           T* H /* may alias X or R */, void* Y, int64_t ldy,
                                                           uint8_t* __restrict__ S, int64_t lds, float* __restrict__ RSTD,
-                                                          int64_t rows, int ncols, double inv_n, float eps) {
+                                                          int64_t rows, int ncols, double inv_n, typename NormMath<OUT>::type eps) {
     constexpr int G = 256 / LPR;
     typedef typename NormMath<OUT>::type M;
     __shared__ M red[4];
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
         __syncthreads();
         ss = (red[0] + red[1]) + (red[2] + red[3]);
     }
-    const M rstd = inverse_root(mean_of(ss, ncols, inv_n) + (M)eps);
+    const M rstd = inverse_root(mean_of(ss, ncols, inv_n) + eps);
     const float hi = (float)rstd, lo = low_part(rstd, hi);
     if (row_ok && l == 0) RSTD[row] = hi;
 #pragma unroll
@@ -150,7 +151,8 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(const T* X, const T* R
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, const T* R, const void* __restrict__ W, int w_dt,
                                                                   T* H, void* Y, int64_t ldy, uint8_t* __restrict__ S, int64_t lds,
-                                                                  float* __restrict__ RSTD, int64_t rows, int ncols, double inv_n, float eps) {
+                                                                  float* __restrict__ RSTD, int64_t rows, int ncols, double inv_n,
+                                                                  typename NormMath<OUT>::type eps) {
     typedef typename NormMath<OUT>::type M;
     __shared__ M red[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -173,7 +175,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, co
     ss = group_sum<64>(ss);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
-    const M rstd = inverse_root(mean_of((red[0] + red[1]) + (red[2] + red[3]), ncols, inv_n) + (M)eps);
+    const M rstd = inverse_root(mean_of((red[0] + red[1]) + (red[2] + red[3]), ncols, inv_n) + eps);
     const float hi = (float)rstd, lo = low_part(rstd, hi);
     if (tid == 0) RSTD[row] = hi;
     for (int b = wave; b < blocks; b += 4) {
@@ -206,19 +208,19 @@ __global__ __launch_bounds__(256) void add_rmsnorm_generic_kernel(const T* X, co
 
 template <typename T, int OUT>
 static void launch_add_rmsnorm(const void* x, const void* r, const void* w, int w_dt, void* h, void* y, int64_t ldy, void* s,
-                               int64_t lds, float* rstd, int64_t rows, int ncols, float eps, hipStream_t stream) {
+                               int64_t lds, float* rstd, int64_t rows, int ncols, double eps, hipStream_t stream) {
     const T *X = (const T*)x, *R = (const T*)r;
     T* H = (T*)h;
 #define GO_TAIL(L, V, TAIL_)                                                                                         \
     add_rmsnorm_kernel<T, L, V, OUT, TAIL_><<<dim3((unsigned)((rows + 256 / L - 1) / (256 / L))), 256, 0, stream>>>( \
-        X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, eps)
+        X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, (typename NormMath<OUT>::type)eps)
 #define GO(L, V)                                                                                                     \
     do {                                                                                                             \
         if (ncols % 8) GO_TAIL(L, V, true);                                                                          \
         else GO_TAIL(L, V, false);                                                                                   \
     } while (0)
     if (ncols > 16384)
-        add_rmsnorm_generic_kernel<T, OUT><<<dim3((unsigned)rows), 256, 0, stream>>>(X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, eps);
+        add_rmsnorm_generic_kernel<T, OUT><<<dim3((unsigned)rows), 256, 0, stream>>>(X, R, w, w_dt, H, y, ldy, (uint8_t*)s, lds, rstd, rows, ncols, 1.0 / ncols, (typename NormMath<OUT>::type)eps);
     else if (ncols <= 128) GO(16, 1);
     else if (ncols <= 256) GO(32, 1);
     else if (ncols <= 512) GO(64, 1);
@@ -236,7 +238,7 @@ static void launch_add_rmsnorm(const void* x, const void* r, const void* w, int 
 using namespace fx;
 
 extern "C" int fx_add_rmsnorm_fwd(const void* x, const void* residual, const void* w, void* h, void* y, int64_t ldy, void* s,
-                                  int64_t lds, float* rstd, int64_t rows, int ncols, float eps, int x_dt, int w_dt, int y_dt,
+                                  int64_t lds, float* rstd, int64_t rows, int ncols, double eps, int x_dt, int w_dt, int y_dt,
                                   hipStream_t stream) {
     if (rows < 0 || ncols <= 0) FX_FAIL("fx_add_rmsnorm_fwd: bad shape rows=%lld ncols=%d", (long long)rows, ncols);
     if (x_dt != DT_F32 && x_dt != DT_F16 && x_dt != DT_BF16) FX_FAIL("fx_add_rmsnorm_fwd: unsupported dtype enum %d", x_dt);

@@ -503,9 +503,10 @@ int compute_buf_size(int T, int N, int k, const double* compute, const double* d
  * NULL); h may be x or residual.  w: (ncols,) of dtype w_dt or NULL.  rstd: fp32 (rows,).
  * y_dt == x_dt: y (rows, ncols) contiguous, rounded as fx_rmsnorm_fwd rounds; s is not used.
  * y_dt FX_DT_E4M3 / FX_DT_E5M2: y holds 8-bit rows ldy apart (ldy = ncols rounded up to 16, the bytes in
- * between are written as 0), s the scale bytes, of row r and columns [128 b, 128 b + 128) at s[b * lds + r]. */
+ * between are written as 0), s the scale bytes, of row r and columns [128 b, 128 b + 128) at s[b * lds + r].
+ * eps is used in 64 bits for an 8-bit output and in 32 for one of x's dtype. */
 int fx_add_rmsnorm_fwd(const void* x, const void* residual, const void* w, void* h, void* y, int64_t ldy, void* s,
-                       int64_t lds, float* rstd, int64_t rows, int ncols, float eps, int x_dt, int w_dt, int y_dt,
+                       int64_t lds, float* rstd, int64_t rows, int ncols, double eps, int x_dt, int w_dt, int y_dt,
                        hipStream_t stream);
 
 /* Gradient of x and residual alike: dx = (dh ? dh : 0) + the norm's gradient of dy, dh being the gradient that

@@ -257,3 +257,21 @@ def test_same_dtype_output_of_other_rows_differs_by_the_order_of_a_sum(dev, cols
     want, rstd = ops.flextrain_rmsnorm_fwd(x, w)
     torch.testing.assert_close(R.double(), rstd.double(), rtol=2.0 ** -17, atol=0)
     torch.testing.assert_close(Y.double(), want.double(), rtol=2 * torch.finfo(dtype).eps + 2.0 ** -16, atol=2.0 ** -23 if dtype == torch.float16 else 0)
+
+
+@pytest.mark.parametrize("cols", [120, 128, 16400])
+def test_8_bit_values_are_those_of_the_given_eps(dev, cols):
+    """Rows whose mean square is about eps, and weights that put every y as near to the middle between two e4m3 values as fp32
+    weights can (2^-25 of it): eps rounded to fp32 moves y by 6e-9 of itself, across the middle in every tenth place."""
+    for seed in range(3):
+        g = gen(20 + seed)
+        h = torch.randn(1, cols, generator=g) * 3e-3
+        rstd = 1 / torch.sqrt((h.double() ** 2).mean() + EPS)
+        middle = (1 + torch.randint(0, 8, (cols,), generator=g) / 8 + 1 / 16).double() * 2.0 ** torch.randint(-3, 0, (cols,), generator=g)
+        middle[::16] = 1.5                     # a block's largest: its scale is 2^-8
+        w = (middle / (h[0].double() * rstd)).float()
+        q, s, _, _ = ops.flextrain_add_rmsnorm_fwd(h.to(dev), None, w.to(dev), output_dtype=o.E4M3, rms_norm_eps=EPS)
+        _, _, y = o.add_rmsnorm(h, None, w, EPS)
+        want, scale = o.quantize(y, o.E4M3)
+        same(s, scale, "scales")
+        same(q, want, "values")
