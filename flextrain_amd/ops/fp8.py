@@ -306,7 +306,8 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
         raise ValueError(f"{op}: A has no rows")
     b_stride = B.stride()
     lda, ldb = _values(A, a_rows, K, A.stride(), "A", op), _values(B, N, K, b_stride, "B", op)
-    if E > 1 and N and K and b_stride[0] % 16:
+    b_expert = b_stride[0] if E > 1 else 0          # (a dimension of one has no stride of its own)
+    if N and K and b_expert % 16:
         raise ValueError(f"{op}: every expert's matrix must start at a 16-byte address")
     sa_row, sa_k, _ = _scales(A_scales, a_rows, kb, False, "A_scales", op)
     if B_scales.dim() != 3 or B_scales.shape[0] != E:
@@ -319,7 +320,7 @@ def flextrain_fp8_grouped_matmul(A, A_scales, B, B_scales, counts, row_sources=N
     with on_device(A):
         rc = lib().fx_fp8_grouped_gemm(A.data_ptr(), lda, a_dt, A_scales.data_ptr(), sa_row, sa_k,
                                        None if row_sources is None else row_sources.data_ptr(), a_rows, B.data_ptr(), ldb,
-                                       b_stride[0], B_scales.data_ptr(), sb_row, sb_k, B_scales.stride(0), b_tiles,
+                                       b_expert, B_scales.data_ptr(), sb_row, sb_k, B_scales.stride(0), b_tiles,
                                        counts.data_ptr(), E, rows, D.data_ptr(), ldd, N, K, d_dt, raw_stream(A))
     check(rc, "fx_fp8_grouped_gemm")
     return D

@@ -524,3 +524,14 @@ def test_host_tensors_are_refused(dev):
         ops.flextrain_fp8_matmul(q, s, q.cpu(), s)
     with pytest.raises(ValueError):
         ops.flextrain_add_rmsnorm_fwd(x.to(dev), x)
+
+
+def test_one_expert_has_no_stride_between_experts(dev):
+    g = gen(17)
+    a, sa, av = operand(dev, values(g, 9, 256))
+    q, s, qv = operand(dev, values(g, 40, 256), tiles=True)
+    counts = torch.tensor([9], dtype=torch.int32).to(dev)
+    want = av @ qv.t()
+    for step in (40 * 256, 40 * 256 + 8, 1, 0):
+        b = q.as_strided((1, 40, 256), (step, 256, 1))
+        check(ops.flextrain_fp8_grouped_matmul(a, sa, b, s[None], counts), want, av, qv, what=f"stride {step}")
