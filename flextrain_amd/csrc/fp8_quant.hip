@@ -356,10 +356,12 @@ extern "C" int fx_fp8_quantize_grouped_cols(const void* x, int64_t ldx, int64_t 
     if (rows < 0 || E <= 0) FX_FAIL("fx_fp8_quantize_grouped_cols: bad shape rows=%lld E=%d", (long long)rows, E);
     const int64_t cap = fx_fp8_grouped_capacity(rows, E);
     if (cap == 0) return 0;
+    // rows of qt are operands of fx_fp8_grouped_wgrad, which takes strides below 2^23
+    if (cap >= (1 << 23)) FX_FAIL("fx_fp8_quantize_grouped_cols: a capacity of %lld rows is not below 2^23", (long long)cap);
     if (!counts || !qt || !st) FX_FAIL("fx_fp8_quantize_grouped_cols: null pointer");
     if (rows > 0 && src_rows == 0) FX_FAIL("fx_fp8_quantize_grouped_cols: the source has no rows");
     if (!row_map && src_rows < rows) FX_FAIL("fx_fp8_quantize_grouped_cols: x has fewer rows than the experts");
-    if (rows > (1 << 24) || src_rows > 0x7fffffff) FX_FAIL("fx_fp8_quantize_grouped_cols: at most 2^24 expert rows");
+    if (src_rows > 0x7fffffff) FX_FAIL("fx_fp8_quantize_grouped_cols: the source has too many rows");
     if ((ldt & 15) || ldt != cap || !aligned16(qt) || ldst < cols)
         FX_FAIL("fx_fp8_quantize_grouped_cols: qt holds %lld values a row, at 16-byte addresses, and its scales %lld", (long long)cap, (long long)cols);
     const int64_t cb = (cols + 127) / 128;

@@ -147,7 +147,8 @@ def flextrain_fp8_quantize_grouped_cols(X, counts, dtype=torch.float8_e4m3fn, ro
     matrix, quantised per expert in blocks of 128 rows of one column.
 
     ``qt`` is ``(cols, capacity)`` with every expert's rows starting at a multiple of 128 (capacity: room for any
-    split of the rows); places without a row hold 0 with scale 1.  ``counts (E,)`` int32 on the GPU.  With
+    split of the rows, ``(rows + 127 E) // 128 * 128``, which has to be below 2**23); places without a row hold 0 with
+    scale 1.  ``counts (E,)`` int32 on the GPU.  With
     ``row_sources`` (int32, one entry per expert-sorted row) ``X`` is the unsorted matrix and sorted row ``r`` is its
     row ``row_sources[r]``."""
     op = "flextrain_fp8_quantize_grouped_cols"
@@ -156,13 +157,13 @@ def flextrain_fp8_quantize_grouped_cols(X, counts, dtype=torch.float8_e4m3fn, ro
     _, x_rows, cols, ldx, _ = _input_matrix(X, op)
     E = _counts_of(counts, op)
     rows = x_rows if row_sources is None else _sources_of(row_sources, op)
+    cap = (rows + 127 * E) // 128 * 128          # fx_fp8_grouped_capacity
+    if cap >= 1 << 23:
+        raise ValueError(f"{op}: the capacity {cap} of {rows} rows and {E} experts is not below 2**23")
     require_same_device(X, counts, row_sources, op=op)
     if rows > 0 and x_rows == 0:
         raise ValueError(f"{op}: X has no rows")
-    if rows > 1 << 24:
-        raise ValueError(f"{op}: at most 2**24 expert rows")
     x_dt, q_dt = dtype_enum(X.dtype), fp8_enum(dtype)
-    cap = (rows + 127 * E) // 128 * 128          # fx_fp8_grouped_capacity
     qt = X.new_empty((cols, cap), dtype=dtype)
     st = _scale_store(X, None, cols, cap // 128)
     if cap > 0:

@@ -540,7 +540,7 @@ int64_t fx_fp8_grouped_capacity(int64_t rows, int E);
  * matrix qt (cols, ldt = fx_fp8_grouped_capacity(rows, E)) in which every expert's rows start at a multiple of
  * 128, with scales per 128 rows of one column at st[b * ldst + c]; places without a row hold 0 with scale 1.
  * row_map (or NULL): sorted row r is row row_map[r] of x, which then has src_rows rows (entries are clamped to
- * them).  At most 2^24 rows. */
+ * them).  ldt, the capacity, has to be below 2^23, as fx_fp8_grouped_wgrad asks of its operands. */
 int fx_fp8_quantize_grouped_cols(const void* x, int64_t ldx, int64_t src_rows, int64_t rows, int64_t cols, int x_dt,
                                  int q_dt, const int32_t* counts, int E, const int32_t* row_map, void* qt, int64_t ldt,
                                  void* st, int64_t ldst, hipStream_t stream);

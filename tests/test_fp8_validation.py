@@ -181,3 +181,20 @@ def test_only_the_two_8_bit_types_have_an_enum():
     for t in (torch.bfloat16, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz, torch.uint8):
         with pytest.raises(TypeError):
             fp8_enum(t)
+
+
+def test_expert_columns_that_no_weight_gradient_takes_are_refused():
+    """Rows of the quantised columns are operands of the expert weight gradient, whose strides are below 2^23."""
+    from flextrain_amd import ops
+
+    cap = lambda rows, E: (rows + 127 * E) // 128 * 128
+    for rows, E in (((1 << 23) - 127, 1), ((1 << 23) - 4 * 127, 4), (1 << 24, 2), (5, 1 << 17)):
+        assert cap(rows, E) >= 1 << 23
+        assert _columns(rows=rows, src=rows, E=E, ldt=cap(rows, E)) == -1
+        with pytest.raises(ValueError, match="capacity"):
+            ops.flextrain_fp8_quantize_grouped_cols(torch.empty(rows, 1, dtype=torch.bfloat16, device="meta"), torch.ones(E, dtype=torch.int32))
+    # the largest that both take: refused only for what is broken beside it
+    rows = (1 << 23) - 128
+    assert cap(rows, 1) < 1 << 23 and _columns(rows=rows, src=rows, E=1, ldt=cap(rows, 1), counts=None) == -1
+    with pytest.raises(ValueError, match="on the GPU"):
+        ops.flextrain_fp8_quantize_grouped_cols(torch.empty(rows, 1, dtype=torch.bfloat16, device="meta"), torch.ones(1, dtype=torch.int32))
