@@ -385,6 +385,15 @@ struct Fp8Loop {
     }
 };
 
+// What the lanes of a wave have written to LDS, its other lanes may read from here on (and overwrite what was read).  The LDS
+// serves a wave's accesses in their order, so this is no instruction: it keeps the compiler, which sees one lane's
+// addresses, from exchanging them.
+FX_DEV void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // D (+ C) of one wave from its accumulators, a band of 32 rows at a time through 4 KB of LDS of its own (`st`), so that a
 // load or store instruction of a wave covers eight whole 128-byte pieces of rows.
 //   accumulator side  lane (r, h) = (lane % 32, lane / 32) holds of row 32 i + r the columns 32 j + 8 g + 4 h .. + 3
@@ -438,12 +447,12 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
         if (LAND && i == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int s = 0; s < PASS; ++s) {
-            // lockstep: the previous band has been read back before this one is staged
+            wave_exchange();          // the previous band has been read back before this one is staged
             if (C != nullptr) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) *at(t * 8 + rr, ch) = c[i % CB][s][t];
             }
-            // lockstep: a wave reads back only what it wrote itself; its LDS accesses complete in order
+            wave_exchange();
 #pragma unroll
             for (int jj = 0; jj < JP; ++jj)
 #pragma unroll
@@ -471,7 +480,7 @@ FX_DEV void fp8_epilogue(const f32x16_t (&acc)[TM][TN], const TD* C, int64_t ldc
                         *p = o;
                     }
                 }
-            // lockstep: as above
+            wave_exchange();
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 const Pack o = *at(t * 8 + rr, ch);

@@ -198,3 +198,18 @@ def test_expert_columns_that_no_weight_gradient_takes_are_refused():
     assert cap(rows, 1) < 1 << 23 and _columns(rows=rows, src=rows, E=1, ldt=cap(rows, 1), counts=None) == -1
     with pytest.raises(ValueError, match="on the GPU"):
         ops.flextrain_fp8_quantize_grouped_cols(torch.empty(rows, 1, dtype=torch.bfloat16, device="meta"), torch.ones(1, dtype=torch.int32))
+
+
+def test_lanes_exchange_through_lds_by_a_fence():
+    """The epilogue of the 8-bit tiles hands values from lane to lane through LDS with no workgroup barrier: a fence of the
+    wave's scope orders them in the program (in the host simulation it is what brings the lanes together)."""
+    import os
+
+    import flextrain_amd
+
+    text = open(os.path.join(os.path.dirname(flextrain_amd.__file__), "csrc", "fp8_core.h")).read()
+    assert "// lockstep:" not in text                                       # an order that only a comment claims
+    body = text[text.index("FX_DEV void wave_exchange()"):][:400]
+    assert body.index("__ATOMIC_RELEASE") < body.index("wave_barrier()") < body.index("__ATOMIC_ACQUIRE")
+    epilogue = text[text.index("FX_DEV void fp8_epilogue"):text.index("kernels over a list of tiles")]
+    assert epilogue.count("wave_exchange();") == 3                          # band free, C staged, band staged
