@@ -42,6 +42,8 @@ def pytest_collection_modifyitems(config, items):
 def pytest_runtest_setup(item):
     """Name every GPU test on the real stderr, flushed, before it touches the card: a run that ends with
     the machine (a fault takes the box and its files along) still shows which test it was in."""
+    if hostsim_mode.ACTIVE:       # a test starts on an idle device: what others left pending on their memory is done
+        hostsim_mode.CLOCKS.host_sync()
     if item.get_closest_marker("gpu") is not None:
         sys.__stderr__.write(f"[gpu test] {item.nodeid}\n")
         sys.__stderr__.flush()

@@ -21,6 +21,8 @@
 #include <functional>
 #include <vector>
 
+#include <malloc.h>
+
 #define __global__
 #define __device__
 #define __host__
@@ -63,6 +65,7 @@ template <typename T> inline hipError_t hipGetSymbolAddress(void** out, T* sym) 
 extern "C" {
 uint64_t hostsim_order_snapshot(uint64_t stream);
 void hostsim_order_wait(uint64_t stream, uint64_t handle);
+void hostsim_order_forget(uint64_t lo, uint64_t bytes);
 int hostsim_order_enqueue(uint64_t stream, const char* what, int n, const uint64_t* lo, const uint64_t* bytes, const int* is_write);
 }
 enum { hipErrorStreamOrder = 2 };
@@ -92,7 +95,11 @@ inline hipError_t hipEventDestroy(hipEvent_t e) { delete e; return hipSuccess; }
 inline hipError_t hipEventRecord(hipEvent_t e, hipStream_t s) { e->snapshot = hostsim_order_snapshot((uint64_t)(uintptr_t)s); return hipSuccess; }
 inline hipError_t hipStreamWaitEvent(hipStream_t s, hipEvent_t e, unsigned) { hostsim_order_wait((uint64_t)(uintptr_t)s, e->snapshot); return hipSuccess; }
 inline hipError_t hipHostMalloc(void** p, size_t n, unsigned) { *p = malloc(n); return *p ? hipSuccess : hipErrorInvalidValue; }
-inline hipError_t hipHostFree(void* p) { free(p); return hipSuccess; }
+inline hipError_t hipHostFree(void* p) {
+    if (p) hostsim_order_forget((uint64_t)(uintptr_t)p, malloc_usable_size(p));
+    free(p);
+    return hipSuccess;
+}
 
 namespace hostsim {
 

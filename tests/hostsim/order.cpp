@@ -13,6 +13,7 @@
 #include <map>
 #include <set>
 #include <string>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -85,6 +86,25 @@ void hostsim_order_host_sync(uint64_t handle) {
 void hostsim_order_stream_sync(uint64_t stream) {
     g_snapshots.push_back(snapshot_of(stream));
     hostsim_order_host_sync(g_snapshots.size() - 1);
+}
+
+// Memory that was released: what was declared for these bytes says nothing about whatever is allocated there next.
+void hostsim_order_forget(uint64_t lo, uint64_t bytes) {
+    const uint64_t hi = lo + bytes;
+    std::vector<Access> kept;
+    for (Access& p : g_history) {
+        if (p.hi <= lo || hi <= p.lo) {
+            kept.push_back(p);
+            continue;
+        }
+        for (const auto& part : {std::make_pair(p.lo, lo), std::make_pair(hi, p.hi)})
+            if (part.first < part.second) {
+                kept.push_back(p);
+                kept.back().lo = part.first;
+                kept.back().hi = part.second;
+            }
+    }
+    g_history.swap(kept);
 }
 
 // One operation on `stream` with n byte ranges (lo[i], bytes[i], is_write[i]).  Returns 0, or 1 when one

@@ -21,7 +21,7 @@ class Clocks:
         for name, restype, argtypes in (("hostsim_order_snapshot", u64, [u64]), ("hostsim_order_wait", None, [u64, u64]),
                                         ("hostsim_order_wait_stream", None, [u64, u64]), ("hostsim_order_host_sync", None, [u64]),
                                         ("hostsim_order_stream_sync", None, [u64]), ("hostsim_order_checked", u64, []),
-                                        ("hostsim_order_deafen", None, [u64]),
+                                        ("hostsim_order_deafen", None, [u64]), ("hostsim_order_forget", None, [u64, u64]),
                                         ("hostsim_order_last_violation", ctypes.c_char_p, [])):
             fn = getattr(handle, name)
             fn.restype, fn.argtypes = restype, argtypes
@@ -42,6 +42,10 @@ class Clocks:
 
     def stream_sync(self, stream):
         self._h.hostsim_order_stream_sync(stream)
+
+    def forget(self, lo, nbytes):
+        """The memory was released: what was declared for it does not hold for what is allocated there next."""
+        self._h.hostsim_order_forget(lo, nbytes)
 
     def deafen(self, stream):
         """For the check's own test: the stream's waits are ignored from now on, as if never made."""

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 import mmap
 import os
+import weakref
 
 import torch
 
@@ -56,6 +57,8 @@ def guard(t: torch.Tensor, align: int = 16, keep: bool = True) -> torch.Tensor:
     start = _PAGE if os.environ.get("HOSTSIM_GUARD_SIDE") == "front" else (_PAGE + body - nbytes) // align * align
     if keep:
         _keep.append(mm)
+    elif _lib is not None:       # the order check forgets what was declared for the pages when they go
+        weakref.finalize(mm, _lib.hostsim_order_forget, ctypes.c_uint64(base + _PAGE), ctypes.c_uint64(body)).atexit = False
     out = torch.frombuffer(mm, dtype=t.dtype, count=t.numel(), offset=start).view(t.shape)
     out.copy_(t)
     return out

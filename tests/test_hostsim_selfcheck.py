@@ -127,3 +127,39 @@ def test_a_removed_wait_in_the_streamed_optimizer_step_is_reported():
         """)
         out = bad.stdout
         assert bad.returncode == 0 and out.count("is not ordered after") == 2 and "returned 0" not in out, (role, out[-900:], bad.stderr[-1500:])
+
+
+def test_the_order_check_forgets_released_memory():
+    """Accesses declared for a tensor of the simulated GPU suite, or for pinned memory, count as long as it lives: what is allocated
+    at its address afterwards is another buffer.  The rest of a range that is released in part still counts."""
+    run = _child("""
+        import os, sys
+        os.environ["FLEXTRAIN_HOSTSIM"] = "1"
+        sys.path.insert(0, "tests")
+        import ctypes
+        import torch
+        from hostsim import mode, sim
+        mode.ACTIVE = True
+        mode.activate()
+        from flextrain_amd.host_memory import LocalPinnedHostBackend
+        u64 = ctypes.c_uint64
+        def write(stream, lo, n):
+            return sim.lib().hostsim_order_enqueue(u64(stream), b"write", 1, (u64 * 1)(lo), (u64 * 1)(n), (ctypes.c_int * 1)(1))
+        pinned = LocalPinnedHostBackend()
+        for allocate, release in ((lambda: torch.zeros(5000, dtype=torch.uint8, device="cuda"), lambda t: None),
+                                  (lambda: pinned.allocate_tensor((5000,), torch.uint8), pinned.release)):
+            t = allocate()
+            lo = t.data_ptr()
+            assert write(0x10, lo, 5000) == 0
+            assert write(0x20, lo + 100, 8) == 1             # alive, and not ordered after the first
+            release(t)
+            del t
+            assert write(0x30, lo, 5000) == 0
+        mode.CLOCKS.host_sync()
+        assert write(0x10, 1 << 20, 300) == 0
+        mode.CLOCKS.forget((1 << 20) + 100, 100)
+        assert write(0x20, (1 << 20) + 100, 100) == 0
+        assert write(0x30, (1 << 20) + 99, 1) == 1 and write(0x30, (1 << 20) + 200, 1) == 1
+        print("fine")
+    """)
+    assert run.returncode == 0 and "fine" in run.stdout, run.stderr[-2000:]
