@@ -112,6 +112,8 @@ def activate():
     from . import sim
 
     global CLOCKS
+    # the simulated kernels run on one thread; the workers of a test run share the cores between them
+    torch.set_num_threads(min(2, torch.get_num_threads()))
     _lib._lib = sim.lib()
     CLOCKS = order.Clocks(sim.lib())
     default = _Stream()
