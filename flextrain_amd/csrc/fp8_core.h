@@ -743,7 +743,14 @@ __global__ __launch_bounds__(NW * 64) void fp8_small_kernel(Source src) {
 
 // ---------------------------------------------------------------- which kernel
 // Times in microseconds, fitted to sweeps of M in 1 .. 2048, N and K in 1000 .. 14336 (dense) and of 8 .. 65536 rows over
-// 128 experts (within 15 % of what was measured except where the weights' bytes bind every form alike):
+// 128 experts.  They are for choosing, and good to a factor of 1.5 either way, not better: over 241 dense products (M 16 ..
+// 6373, N 128 .. 14336, K 256 .. 11915) the measured time is 0.76 to 1.51 of the fit in nine of ten, within 15 % in 60 of 100;
+// over 179 by expert (8 .. 128 experts of 1 .. 512 rows on average) 0.85 to 1.49, within 15 % in 44 of 100.  Operands that the
+// caches do not hold (6373 x 344 x 11915: 84 measured, 52 fitted; 333 x 14336 x 11915: 122, 72) and 128-row tiles at two
+// and more to a CU are slower than fitted, the smallest launches faster.  What the choice costs against the fastest of the three
+// forms: nothing in half of the dense products, up to 6 % in nine of ten, at worst 1.6 times (333 x 579 x 256: 6.0 us in 128 x 128
+// tiles, 3.7 small; 1024 x 579 x 4096: 25.6 small, 19.1 in tiles); by expert up to 9 % in nine of ten, at worst 1.5
+// times (32 experts of 128 rows, N 2048, K 768: 29.9 us in 256-row tiles, 19.6 in 128-row ones: the rows are not split evenly).
 //   small   4 + max(1, workgroups / 256) * steps * (MT + NT) * 0.05 + 5 for every million outputs      a CU takes in 40 KB of
 //           operands per us; its stores are 8 bytes a lane
 //   128     4 + steps * 0.62 up to one workgroup per CU, 0.95 at two, then steps * 1.1 + 3 for every further 512
@@ -765,7 +772,12 @@ static inline double fp8_time_128(double workgroups, double steps) {
 }
 static inline double fp8_time_256(double tiles, double steps) { return 4.0 + ceil(tiles / 256.0) * (steps * 1.5 + 5.0); }
 
-// Waves and K-steps in flight of the small kernel: the four forms that were fastest for their tile.
+// Waves that share a tile's contraction (4 or 8) and K-steps each has in flight (1, 2 or 4) in the small kernel.  Few operands per step
+// leave registers for more of them in flight; the 64 KB of sums of a 4 x 4 tile leave room for 4 waves.  Measured over the
+// products for which a tile is within 25 % of the fastest (M 1 .. 1000, N 579 .. 14336, K 1000 .. 4096; 8 x 2: 8 waves, 2 in
+// flight), the other settings against the one taken, on average: 1 x 1 (8 x 4) 0.97 .. 1.01;  1 x 2 (8 x 2) 1.02 .. 1.11;
+// 1 x 4 (8 x 2) 1.00 .. 1.08;  2 x 2 (4 x 2) 0.98 .. 1.24;  2 x 4 (4 x 2) 0.98 .. 1.41;  4 x 2 (8 x 1) 0.99 .. 1.38;
+// 4 x 4 (4 x 1) 1.24.
 template <int MT, int NT> struct Fp8SmallShape { static constexpr int NW = (MT == 2 || NT * MT == 16) ? 4 : 8, U = MT * NT == 1 ? 4 : MT == 4 ? 1 : 2; };
 
 static inline int fp8_cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }

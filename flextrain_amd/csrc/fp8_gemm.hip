@@ -96,7 +96,8 @@ __global__ __launch_bounds__(256) void fp8_split_reduce_kernel(const float* __re
 struct Fp8Plan { int tile, small, splits, k_slice; };      // tile 256, 128, or 0: the small kernel's form `small`
 
 // The fastest form by the times of fp8_core.h; 128-row tiles may cut the contraction into slices (blockIdx over tile and
-// slice), which costs a second launch and 4 bytes an element and slice through memory.
+// slice), which costs a second launch and 4 bytes an element and slice through memory: 1, 2, 4, .. slices of four K-steps or
+// more, while tiles and slices fit two to a CU.
 static Fp8Plan fp8_plan(int M, int N, int K) {
     const int steps = fp8_cdiv(K, FP8_BK);
     Fp8Plan best{0, 0, 1, K};

@@ -76,9 +76,10 @@ struct Fp8GroupedWgrad {
 
 struct Fp8RowsPlan { int shift, small; };      // tile rows (their logarithm): 8, 7, or 4 .. 6 with the small kernel's form `small`
 
-// The fastest form by the times of fp8_core.h for rows split evenly over the experts that have any, half a tile of
-// padding each.  (Measured on 128 experts, N 1536, K 2048, routed counts: 8 rows an expert small 1 x 4 73 us, 128 81;
-// 16 rows 94, 82; 64 rows 128 92, 256 100; 128 rows 125, 116; 512 rows 310, 269.)
+// The fastest form by the times of fp8_core.h for rows split evenly over the experts that have any, half a tile of padding
+// each (the split itself is on the device; what that costs stands there).  Measured on 128 experts, N 1536, K 2048,
+// routed counts: 8 rows an expert small 1 x 4 73 us, 128 81; 16 rows 94, 82; 64 rows 128 92, 256 100; 128 rows 125, 116;
+// 512 rows 310, 269.
 static Fp8RowsPlan fp8_rows_plan(int64_t rows, int E, int N, int K) {
     const double live = (double)(E < rows ? E : rows), avg = (double)rows / live;
     const int steps = fp8_cdiv(K, FP8_BK);
@@ -176,6 +177,10 @@ template <int AF, typename TD>
 static int launch_wgrad(const Fp8View& a, const Fp8View& b, const int32_t* counts, int E, int64_t capacity, const TD* C, int64_t ldc,
                         int64_t c_expert, TD* D, int64_t ldd, int64_t d_expert, hipStream_t stream) {
     const int M = a.ext, N = b.ext;
+    // 256 x 256 tiles from three quarters of a round of the 256 CUs on.  Their time against 128 x 128 ones (5 shapes of 256 x 256 to
+    // 1536 x 2048, 1 .. 128 experts of 32 .. 8192 rows on average): up to 64 tiles 1.5 .. 2.3, 96 and 128 tiles 1.4 .. 1.7, 192 tiles
+    // 0.76 .. 1.18 (long contractions gain), whole rounds (256, 512, 768 tiles) 0.82 .. 1.03, a last round that is half full or
+    // less (384, 576) 1.00 .. 1.18.
     const int64_t big = (int64_t)E * fp8_cdiv(M, 256) * fp8_cdiv(N, 256);
     if (big >= 192) {
         typedef Fp8GroupedWgrad<TD, 256, 256> Source;
