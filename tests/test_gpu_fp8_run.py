@@ -380,3 +380,20 @@ def test_outputs_that_overlap_are_refused(dev):
     wide = torch.zeros(16, 2, 16, dtype=torch.bfloat16, device=dev)
     ops.flextrain_fp8_grouped_wgrad(a, sa, b, sb, counts, C=one.expand(2, 16, 16), out=wide.transpose(0, 1))
     assert (wide == 1.0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(384, 200), (300, 136), (5, 64)])
+def test_columns_alone_are_those_of_one_expert(dev, rows, cols):
+    """A weight gradient reads the columns of the norm's output and nothing of its rows: all rows as one expert's."""
+    g = gen(rows)
+    y, dout = values(g, rows, cols).to(dev), values(g, rows, 72, sigma=1e-3).to(dev)
+    all_rows = torch.tensor([rows], dtype=torch.int32).to(dev)
+    yt, yts = ops.flextrain_fp8_quantize_grouped_cols(y, all_rows)
+    _, _, want, want_s = ops.flextrain_fp8_quantize_both(y)
+    same(yt[:, :rows], want.cpu().float().double(), "values")
+    same(yts, want_s.cpu().float().double(), "scales")
+    assert (yt.float()[:, rows:] == 0).all()
+    _, _, dt, dts = ops.flextrain_fp8_quantize_both(dout, dtype=E5M2)
+    dw = torch.randn(72, cols, generator=g).to(torch.bfloat16).to(dev)
+    got = ops.flextrain_fp8_matmul(dt, dts, yt[:, :rows], yts, C=dw)
+    assert torch.equal(got, ops.flextrain_fp8_matmul(dt, dts, want, want_s, C=dw))
