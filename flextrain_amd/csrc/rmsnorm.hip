@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_generic_kernel(
 // ANY: rows at any address and of any length (a last pack of 1 .. 7 values is read, and written, one by one).
 template <typename T, int LPR, int MAXV, int THREADS, bool ANY>
 __global__ __launch_bounds__(THREADS) void rmsnorm_bwd_kernel(
-    const T* __restrict__ DY, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
+    const T* DY /* may be DX */, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
     const float* __restrict__ RSTD, T* DX, const T* OLD /* added to dx; may be DX; or null */, T* __restrict__ YOUT,
     float* __restrict__ PARTIAL /* [gridDim.x][ncols] or null */, int64_t rows, int ncols,
     int iters) {
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256) void rmsnorm_dw_reduce_kernel(
 // Any-shape fallback backward: one workgroup per row for dx/y ...
 template <typename T>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_generic_kernel(
-    const T* __restrict__ DY, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
+    const T* DY /* may be DX */, const T* __restrict__ X, const void* __restrict__ W, int w_dt,
     const float* __restrict__ RSTD, T* DX, const T* OLD /* added to dx; may be DX; or null */, T* __restrict__ YOUT,
     int64_t rows, int ncols) {
     __shared__ float red[4];
@@ -554,11 +554,7 @@ static int rmsnorm_bwd(bool any, const void* dy, const void* x, const void* w, c
             FX_FAIL("fx_rmsnorm_bwd: workspace too small (%zu < %zu bytes)", ws_bytes, need);
     }
     if (!vec && !odd) {
-        FX_DISPATCH_DTYPE(x_dt, T,
-            rmsnorm_bwd_generic_kernel<T><<<dim3((unsigned)rows), 256, 0, stream>>>(
-                reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), w, w_dt, rstd,
-                reinterpret_cast<T*>(dx), reinterpret_cast<const T*>(old), reinterpret_cast<T*>(y_out), rows, ncols));
-        FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dx)");
+        // dw first: dx may be written over dy
         if (want_dw && any) {
             const int band = dw_band(rows), bands = dw_bands(rows);
             FX_DISPATCH_DTYPE(x_dt, T,
@@ -578,6 +574,11 @@ static int rmsnorm_bwd(bool any, const void* dy, const void* x, const void* w, c
                         reinterpret_cast<TDW*>(dw), accumulate_dw, rows, ncols)));
             FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dw)");
         }
+        FX_DISPATCH_DTYPE(x_dt, T,
+            rmsnorm_bwd_generic_kernel<T><<<dim3((unsigned)rows), 256, 0, stream>>>(
+                reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(x), w, w_dt, rstd,
+                reinterpret_cast<T*>(dx), reinterpret_cast<const T*>(old), reinterpret_cast<T*>(y_out), rows, ncols));
+        FX_CHECK_LAUNCH("fx_rmsnorm_bwd(generic dx)");
         return 0;
     }
     const int groups = bwd_threads(c) / c.lpr;

@@ -191,7 +191,7 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
     and of ``residual`` alike.
 
     ``dH`` is the gradient that reaches ``H`` past the norm (the residual stream's; ``None``: zero) and is left as it is
-    unless it is given as ``dX`` too.  ``dY`` is the gradient of the unquantised output (the 8-bit rounding is passed
+    unless it is given as ``dX`` too; ``dY``, ``dH`` and ``dX`` may be one tensor.  ``dY`` is the gradient of the unquantised output (the 8-bit rounding is passed
     straight through).  ``dW``: accumulated into when given, else a fresh fp32 gradient; ``None`` without ``W``."""
     op = "flextrain_add_rmsnorm_bwd"
     shape, dtype = H.shape, H.dtype

@@ -510,7 +510,7 @@ int fx_add_rmsnorm_fwd(const void* x, const void* residual, const void* w, void*
                        hipStream_t stream);
 
 /* Gradient of x and residual alike: dx = (dh ? dh : 0) + the norm's gradient of dy, dh being the gradient that
- * reaches h past the norm (dx may be dh).  dw (ncols,) of dtype dw_dt or NULL, accumulated into or overwritten;
+ * reaches h past the norm (dx may be dh, dy or both).  dw (ncols,) of dtype dw_dt or NULL, accumulated into or overwritten;
  * ws: fx_add_rmsnorm_bwd_ws_bytes bytes when dw is asked for. */
 size_t fx_add_rmsnorm_bwd_ws_bytes(int64_t rows, int ncols);
 int fx_add_rmsnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx,

@@ -275,3 +275,17 @@ def test_8_bit_values_are_those_of_the_given_eps(dev, cols):
         want, scale = o.quantize(y, o.E4M3)
         same(s, scale, "scales")
         same(q, want, "values")
+
+
+@pytest.mark.parametrize("rows,cols", [(9, 136), (40, 511), (3, 4096), (30, 16387), (5, 16392)])
+def test_backward_with_one_gradient_for_everything(dev, rows, cols):
+    """The gradient that reaches h past the norm may be the norm's own (h used twice), and take the result in its place."""
+    g = gen(rows + cols)
+    h, d = values(g, rows, cols), values(g, rows, cols, sigma=0.5)
+    w = (1 + 0.1 * torch.randn(cols, generator=g)).to(torch.bfloat16).to(dev)
+    _, _, H, rstd = ops.flextrain_add_rmsnorm_fwd(h.to(dev), None, None)
+    dx, dw = ops.flextrain_add_rmsnorm_bwd(d.to(dev), H, w, rstd, dH=d.to(dev))
+    one = d.to(dev)
+    got, dw2 = ops.flextrain_add_rmsnorm_bwd(one, H, w, rstd, dH=one, dX=one)
+    assert got is one and torch.equal(got, dx)
+    assert torch.equal(dw2, dw)
