@@ -53,10 +53,10 @@ FX_DEV double inverse_root(double m) {
     }
     return r;
 }
-// h * (hi + lo) * w to fp32 by rounding to odd (Boldo and Melquiond, IEEE Trans. Computers 57, 2008): of the two neighbours of a value between them the one whose last bit is 1.  It lies on
-// the same side of every 8-bit value, and of every middle between two, as the value itself, so rounding it again gives what
-// rounding the value gives.  Products and their remainders by fma: off by 2^-45 of the value or less (while it is far from
-// fp32's subnormals).
+// h * (hi + lo) * w to fp32 by rounding to odd (Boldo and Melquiond, IEEE Trans. Computers 57, 2008): of the two neighbours of
+// a value between them the one whose last bit is 1.  It lies on the same side of every 8-bit value, and of every middle
+// between two, as the value itself, so rounding it again gives what rounding the value gives.  Products and their
+// remainders by fma: off by 2^-45 of the value or less (while it is far from fp32's subnormals).
 FX_DEV float product_odd(float h, float hi, float lo, float w) {
 #pragma clang fp contract(off)
     const float p = h * hi, pe = fmaf(h, lo, fmaf(h, hi, -p));

@@ -144,10 +144,13 @@ def flextrain_add_rmsnorm_fwd(X, residual=None, W=None, output_dtype=None, sum_o
     ``H = X + residual`` rounded to ``X``'s dtype (``X`` itself without a residual), ``rstd (T, 1)`` fp32 of ``H``,
     ``Y = H * rstd * W``.  ``output_dtype``: ``torch.float8_e4m3fn`` / ``torch.float8_e5m2`` give ``Y`` in 8 bits with
     ``scales (T, ceil(D / 128))`` as :func:`flextrain_fp8_quantize` defines them (``Y`` is formed exactly and rounded
-    once); ``None`` gives ``Y`` in ``X``'s dtype, with the roundings of ``flextrain_rmsnorm_fwd(H, W)``, and no
-    scales: the same ``rstd`` as that op's, and in bf16 and fp32 the same ``Y``, bit for bit, where ``D`` is a multiple of 8
-    and at most 16384 and its tensors start at 16-byte addresses.  Elsewhere that op adds the squares in another order and
-    ``rstd`` may differ in its last bits; in fp16 either op may round a product to fp32 before it rounds it to fp16.  ``sum_out`` receives ``H`` and may be ``X`` or ``residual``."""
+    once); ``None`` gives ``Y`` in ``X``'s dtype, with the roundings of ``flextrain_rmsnorm_fwd(H, W)``, and no scales.
+    ``sum_out`` receives ``H`` and may be ``X`` or ``residual``.
+
+    Against ``flextrain_rmsnorm_fwd(H, W)``: the same ``rstd``, and in bf16 and fp32 the same ``Y``, bit for bit, where
+    ``D`` is a multiple of 8 and at most 16384 and all tensors start at 16-byte addresses.  Elsewhere that op adds the
+    squares in another order and ``rstd`` may differ in its last bits; in fp16 either op may round a product to fp32
+    before it rounds it to fp16."""
     op = "flextrain_add_rmsnorm_fwd"
     shape, dtype = X.shape, X.dtype
     if len(shape) != 2 or not X.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
@@ -191,8 +194,9 @@ def flextrain_add_rmsnorm_bwd(dY, H, W, rstd, dH=None, dX=None, dW=None):
     and of ``residual`` alike.
 
     ``dH`` is the gradient that reaches ``H`` past the norm (the residual stream's; ``None``: zero) and is left as it is
-    unless it is given as ``dX`` too; ``dY``, ``dH`` and ``dX`` may be one tensor.  ``dY`` is the gradient of the unquantised output (the 8-bit rounding is passed
-    straight through).  ``dW``: accumulated into when given, else a fresh fp32 gradient; ``None`` without ``W``."""
+    unless it is given as ``dX`` too; ``dY``, ``dH`` and ``dX`` may be one tensor.  ``dY`` is the gradient of the
+    unquantised output (the 8-bit rounding is passed straight through).  ``dW``: accumulated into when given, else a
+    fresh fp32 gradient; ``None`` without ``W``."""
     op = "flextrain_add_rmsnorm_bwd"
     shape, dtype = H.shape, H.dtype
     if len(shape) != 2 or not H.is_contiguous() or (W is not None and (W.shape != shape[1:] or not W.is_contiguous())):
